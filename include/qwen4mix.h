@@ -50,6 +50,10 @@ extern "C" {
 #define QM_ACT_F32 0
 #define QM_ACT_BF16 1
 
+/* weights of qm_moe: tiles of the activations' type, or of 4-bit codes */
+#define QM_W_ACT 0
+#define QM_W_MX4 1
+
 #define QM_GEMV_MAX_SEG 8
 
 /* Last error message of the calling thread ("" after success). */
@@ -462,6 +466,119 @@ int qm_hc_mix_as(const qm_hc_geom* g, int as_rows, const void* hyper, const floa
  * streams, hidden and act_dtype of g (hidden a multiple of 8). */
 int qm_hc_reinject(const qm_hc_geom* g, const void* hyper, const void* branch, const void* inject, void* out,
                    hipStream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Microscaled 4-bit weights                                                */
+/* ------------------------------------------------------------------------ */
+
+/* A weight matrix [n, k] (k a multiple of 32) in microscaled 4-bit floating
+ * point: E2M1 elements in blocks of 32 along k, one power-of-two scale byte
+ * (2^(byte - 127); 255 is NaN) per block. In memory it is two arrays of tiles
+ * of 16 rows x 128 k, [matrix][ceil(n/16)][ceil(k/128)]: codes of 1024 bytes a
+ * tile, where 16-byte slot l holds block l / 16 of row l % 16 (element j in
+ * nibble j, the low nibble of a byte first), and scales of 64 bytes a tile, byte
+ * l for slot l. Slots past n or k are zero. codes are 16-byte aligned. */
+
+/* Bytes of the codes of `mats` matrices (the scales take a 16th of it); 0 if the
+ * sizes are unsupported. */
+size_t qm_mx4_code_bytes(int mats, int n, int k);
+
+/* Quantise w [mats, n, k] (act_dtype, row-major, 16-byte aligned): a block's
+ * scale is 2^max(floor(log2 max|w|) - 2, -127), its elements w / scale to the
+ * nearest E2M1 value, ties to the even code, magnitudes above 6 to 6. A block
+ * with a NaN or an infinity gets scale 255; one of zeros scale 0. */
+int qm_mx4_quantize(int act_dtype, int mats, int n, int k, const void* w, void* codes, void* scales,
+                    hipStream_t stream);
+
+/* The values they stand for, w [mats, n, k] (act_dtype; every finite value is
+ * exact in either type). */
+int qm_mx4_dequantize(int act_dtype, int mats, int n, int k, const void* codes, const void* scales, void* w,
+                      hipStream_t stream);
+
+/* Between the tiles and the plain order of a checkpoint: plain_codes
+ * [mats, n, k / 2] (16-byte aligned), plain_scales [mats, n, k / 32]; into the
+ * tiles when to_tiles, else out of them. */
+int qm_mx4_layout(int to_tiles, int mats, int n, int k, void* codes, void* scales, void* plain_codes,
+                  void* plain_scales, hipStream_t stream);
+
+/* The projections of qm_gemv / qm_gemm_rows with 4-bit weights, for any number of
+ * activation rows: y[m][j] = sum_k w[j][k] x[m][k], w the values the codes stand
+ * for, float sums rounded once to act_dtype.
+ *   x [m, k] act_dtype, rows ldx elements apart (ldx >= k, whole 16-byte units;
+ *   x 16-byte aligned); segments as qm_gemv. Outputs may not overlap x. */
+int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* codes, const void* scales, const void* x, long ldx,
+                  int n_seg, const int* seg_rows, void* const* seg_out, hipStream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Mixture of experts                                                       */
+/* ------------------------------------------------------------------------ */
+
+/* The routing of the mixture-of-experts layer (reference/model.py:387-417):
+ * logits = x router^T summed in double; ids [rows, top_k] the experts of the
+ * largest logits in falling order (equal logits: the lower index first; NaN
+ * above every number); weights [rows, top_k] their softmax over all experts, or
+ * over the chosen ones when `normalize`.
+ *   x [rows, hidden] act_dtype, rows ldx elements apart; router [experts,
+ *   hidden]; both 16-byte aligned, hidden a multiple of 32, ldx whole 16-byte
+ *   units; experts <= 1024, top_k <= 32. The workspace holds nothing between
+ *   calls. */
+size_t qm_moe_route_workspace(int rows, int experts);
+int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, int normalize, const void* x, long ldx,
+                 const void* router, int* ids, float* weights, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream);
+
+/* bf16 or float weights [mats, n, k] (row-major) into tiles of 16 rows x 128 k,
+ * [mats][ceil(n/16)][ceil(k/128)], zeros past n and k: slot l of a tile holds k
+ * 32 (l / 16) .. + 31 of row l % 16, its 16-byte pieces 1024 bytes apart (4 of
+ * bf16, 8 of float). Both 16-byte aligned, k a multiple of 32. */
+int qm_tile_weight(int act_dtype, int mats, int n, int k, const void* w, void* tiles, hipStream_t stream);
+
+typedef struct qm_moe_geom {
+  int rows;          /* tokens                                               */
+  int hidden;        /* width of x and out (a multiple of 32)                 */
+  int inter;         /* hidden units of an expert (a multiple of 32)          */
+  int experts;       /* routed experts, <= 1024                               */
+  int shared;        /* experts that every token takes, 0..32                 */
+  int top_k;         /* routed experts of a token, <= 32                      */
+  int normalize;     /* the chosen experts' weights add up to 1               */
+  int act_dtype;     /* QM_ACT_F32 or QM_ACT_BF16                             */
+  int weight_format; /* QM_W_ACT (qm_tile_weight) or QM_W_MX4                 */
+} qm_moe_geom;
+
+/* gate, up [experts, inter, hidden] and down [experts, hidden, inter] as tiles
+ * (scales: the 4-bit format's, else unused); router [experts, hidden] act; the
+ * shared experts' likewise when geom.shared, and their gate's row shared_router
+ * [hidden] act or NULL for a weight of 1. */
+typedef struct qm_moe_weights {
+  const void* router;
+  const void* gate;
+  const void* up;
+  const void* down;
+  const void* gate_scales;
+  const void* up_scales;
+  const void* down_scales;
+  const void* shared_router;
+  const void* shared_gate;
+  const void* shared_up;
+  const void* shared_down;
+  const void* shared_gate_scales;
+  const void* shared_up_scales;
+  const void* shared_down_scales;
+} qm_moe_weights;
+
+/* Bytes of workspace qm_moe needs; 0 if the geometry is unsupported. */
+size_t qm_moe_workspace(const qm_moe_geom* g);
+
+/* A whole mixture-of-experts layer (reference/model.py:387-417):
+ *   out[t] = sum_j w[t][j] down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][j]
+ *          + sigmoid(x[t] . shared_router) sum_s (the same of shared expert s)
+ * with ids and w as qm_moe_route. Products accumulate in float; a pair's weighted
+ * hidden row is rounded to act_dtype between them, the output once.
+ *   x [rows, hidden] act, rows ldx elements apart; out [rows, hidden] act; every
+ *   pointer 16-byte aligned. out may not overlap x. The workspace holds nothing
+ *   between calls; calls that overlap need one each. */
+int qm_moe(const qm_moe_geom* g, const qm_moe_weights* w, const void* x, long ldx, void* out, void* workspace,
+           size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,240 @@
+"""Routing (moe_route) and the mixture-of-experts layer (moe) against 64 bits.
+
+The chosen experts are compared exactly (the logits are sums in double on both
+sides; random ones lie far further apart than its rounding). A weight is
+exp(l - max) / sum: the difference is rounded to float (|l - max| < 16 here, so
+2^-20 relative), the exponential, the sum of at most 32 and the division add some
+40 half steps: 2^-18 in all. Outputs are held to the bound of tests/ffn_oracle.py
+and, by norm, to twice half a step of the activations' type: the hidden rows' and
+the output's rounding are independent, each 0.58 half steps in the mean.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import ffn_oracle as fo
+from margins import record
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+W_TOL = 2.0 ** -18
+
+
+def normal(seed, *shape, dtype=F32, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,e,k,h", [(1, 1, 1, 32), (1, 128, 8, 2048), (2, 5, 5, 96), (3, 64, 32, 160), (9, 130, 6, 512),
+                                     (17, 1024, 32, 64), (64, 60, 4, 2080), (333, 256, 10, 256), (1000, 16, 2, 1024)])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_matches_f64(gpu, dtype, t, e, k, h, normalize):
+    x, r = normal(t + e, t, h, dtype=dtype), normal(h, e, h, dtype=dtype, scale=h ** -0.5)
+    ids, w = gpu.moe_route(x, r, k, normalize)
+    want_ids, want_w = fo.route(x, r, k, normalize)
+    assert ids.dtype == torch.int32 and w.dtype == F32 and ids.shape == (t, k)
+    assert torch.equal(ids, want_ids)
+    rel = ((w.double() - want_w).abs() / want_w).max().item()
+    assert record("rel", rel, W_TOL) < W_TOL
+
+
+@pytest.mark.parametrize("t", [1, 6, 70])
+def test_route_ties_and_bad_values(gpu, t):
+    h, e = 64, 12
+    x = normal(1, t, h, dtype=BF16)
+    r = normal(2, e, h, dtype=BF16)
+    r[3] = r[7] = r[9]                                             # equal logits, always
+    ids, w = gpu.moe_route(x, r, e)
+    order = ids[0].tolist()
+    for row in ids.tolist():
+        assert row.index(3) + 1 == row.index(7) and row.index(7) + 1 == row.index(9)
+        assert sorted(row) == list(range(e))
+    assert order == fo.route(x, r, e)[0][0].tolist()
+    zero = torch.zeros_like(x)
+    ids, w = gpu.moe_route(zero, r, 4)                             # every logit equal
+    assert ids.tolist() == [[0, 1, 2, 3]] * t and bool((w == 0.25).all())
+    ids, w = gpu.moe_route(-zero, r, 4)
+    assert ids.tolist() == [[0, 1, 2, 3]] * t
+    x2 = x.clone()
+    x2[0, 5] = float("nan")
+    ids2, w2 = gpu.moe_route(x2, r, 5)
+    assert ids2[0].tolist() == [0, 1, 2, 3, 4] and bool(w2[0].isnan().all())
+    ids, w = gpu.moe_route(x, r, 5)
+    assert torch.equal(ids2[1:], ids[1:]) and torch.equal(w2[1:], w[1:])
+    r2 = r.clone()
+    r2[8, 0] = float("nan")
+    ids3, w3 = gpu.moe_route(x, r2, 2)
+    assert bool((ids3[:, 0] == 8).all()) and bool(w3.isnan().all())
+
+
+def test_route_does_not_depend_on_the_rows_beside(gpu):
+    x, r = normal(5, 300, 512, dtype=BF16), normal(6, 96, 512, dtype=BF16, scale=0.05)
+    ids, w = gpu.moe_route(x, r, 7)
+    for lo, hi in ((0, 1), (4, 6), (10, 27), (100, 260)):
+        part_ids, part_w = gpu.moe_route(x[lo:hi], r, 7)
+        assert torch.equal(part_ids, ids[lo:hi])
+        assert ((part_w.double() / w[lo:hi].double() - 1).abs().max().item()) < W_TOL
+
+
+def layer(qm, seed, e, h, i, shared, top_k, fmt, dtype, gated=True, normalize=True, bias=None):
+    """(MoeWeights, the oracle's arguments)."""
+    router = normal(seed, e, h, dtype=dtype, scale=h ** -0.5)
+    mats = [normal(seed + 1, e, i, h, dtype=dtype, scale=h ** -0.5), normal(seed + 2, e, i, h, dtype=dtype, scale=h ** -0.5),
+            normal(seed + 3, e, h, i, dtype=dtype, scale=i ** -0.5)]
+    sh = None
+    if shared:
+        sh = [normal(seed + 4, shared, i, h, dtype=dtype, scale=h ** -0.5),
+              normal(seed + 5, shared, i, h, dtype=dtype, scale=h ** -0.5),
+              normal(seed + 6, shared, h, i, dtype=dtype, scale=i ** -0.5)]
+    if bias is not None:
+        mats = bias(mats)
+    gate_row = normal(seed + 7, h, dtype=dtype, scale=h ** -0.5) if shared and gated else None
+    if fmt == "mx4":
+        mats = [qm.mx4_quantize(m) for m in mats]
+        sh = None if sh is None else [qm.mx4_quantize(m) for m in sh]
+        values = [m.dequantize().double() for m in mats]
+        sh_values = None if sh is None else [m.dequantize().double() for m in sh]
+    else:
+        values, sh_values = [m.double() for m in mats], None if sh is None else [m.double() for m in sh]
+    w = qm.MoeWeights(router, *mats, top_k=top_k, shared=sh, shared_router=gate_row, normalize=normalize)
+    return w, dict(router=router, gate=values[0], up=values[1], down=values[2], top_k=top_k, normalize=normalize,
+                   shared=sh_values, shared_router=gate_row)
+
+
+def check(got, x, args):
+    want, bound = fo.moe(x, **args)
+    assert got.shape == x.shape and got.dtype == x.dtype
+    assert record("bound", fo.within(got, want, bound, x.dtype), 1.0) <= 1.0
+    rel = ((got.double() - want).norm() / want.norm()).item()
+    lim = 2 * fo.half(x.dtype) if x.dtype == BF16 else 2 ** -19
+    assert record("norm", rel, lim) < lim
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t,e,k,h,i,shared", [(1, 4, 2, 64, 32, 0), (1, 16, 8, 2048, 512, 1), (2, 7, 3, 96, 160, 2),
+                                              (4, 32, 8, 512, 352, 1), (5, 3, 3, 160, 96, 0), (9, 24, 8, 1024, 256, 1),
+                                              (16, 8, 2, 256, 64, 3), (17, 9, 1, 288, 128, 1), (33, 40, 6, 128, 96, 0),
+                                              (70, 12, 4, 544, 224, 1), (260, 6, 3, 256, 128, 1), (300, 64, 8, 128, 64, 2)])
+def test_moe_matches_f64(gpu, dtype, fmt, t, e, k, h, i, shared):
+    print(f"moe {dtype} {fmt} t={t} e={e} k={k} h={h} i={i} shared={shared}", flush=True)
+    w, args = layer(gpu, t + e, e, h, i, shared, k, fmt, dtype, gated=t % 2 == 1, normalize=t % 3 != 0)
+    x = normal(t, t, h, dtype=dtype)
+    check(gpu.moe(x, w), x, args)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t", [1, 3, 12, 64, 500])
+def test_all_tokens_on_few_experts(gpu, fmt, t):
+    """Every token on the same two experts: the others have no rows."""
+    w, args = layer(gpu, 3, 20, 128, 64, 1, 2, fmt, BF16)
+    x = normal(t, t, 128, dtype=BF16, scale=0.1)
+    x += (args["router"][5] + args["router"][17]) * 8
+    got = gpu.moe(x, w)
+    assert set(gpu.moe_route(x, args["router"], 2)[0].flatten().tolist()) == {5, 17}
+    check(got, x, args)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t", [1, 2, 8, 14, 40, 200])
+def test_bad_values_stay_with_their_tokens(gpu, fmt, t):
+    """A token with a NaN is NaN and leaves the others alone; an expert with
+    infinite or NaN weights reaches only the tokens that chose it."""
+    e, k = 10, 2
+
+    def spoil(mats):
+        mats[0][4, 0, 0], mats[2][6, 1, 1], mats[1][6, 2, 2] = float("nan"), float("inf"), float("inf")
+        return mats
+
+    w, args = layer(gpu, 8, e, 96, 64, 1, k, fmt, BF16, bias=spoil)
+    x = normal(t + 50, t, 96, dtype=BF16)
+    ids = gpu.moe_route(x, args["router"], k)[0]
+    got = gpu.moe(x, w)
+    hit = ((ids == 4) | (ids == 6)).any(-1)
+    assert torch.equal(got.isfinite().all(-1), ~hit)
+    x2 = x.clone()
+    x2[t // 2, 7] = float("nan")
+    got2 = gpu.moe(x2, w)
+    assert bool(got2[t // 2].isnan().all())
+    keep = [r for r in range(t) if r != t // 2 and not bool(hit[r])]
+    assert torch.equal(got2[keep], got[keep])
+
+
+@pytest.mark.parametrize("t", [1, 4, 30, 200])
+def test_strides_shapes_streams_and_repeats(gpu, t):
+    w, args = layer(gpu, 11, 16, 128, 96, 1, 4, "mx4", BF16)
+    base = normal(t, t, 300, dtype=BF16)
+    x = base[:, 8:136]                                             # rows 600 bytes apart: copied
+    want = gpu.moe(x.contiguous(), w)
+    check(want, x.contiguous(), args)
+    assert torch.equal(gpu.moe(x, w), want)
+    wide = normal(t, t, 304, dtype=BF16)[:, 16:144]                # rows 608 bytes apart: read in place
+    assert torch.equal(gpu.moe(wide, w), gpu.moe(wide.contiguous(), w))
+    assert torch.equal(gpu.moe(x.reshape(1, t, 1, 128), w).reshape(t, 128), want)
+    assert gpu.moe(x[:0], w).shape == (0, 128)
+    assert all(torch.equal(gpu.moe(x, w), want) for _ in range(3))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = gpu.moe(x, w)
+    here = gpu.moe(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want) and torch.equal(here, want)
+
+
+@pytest.mark.parametrize("t", [1, 7, 90])
+def test_graph_replays(gpu, t):
+    w, args = layer(gpu, 12, 16, 128, 96, 1, 4, "plain", BF16)
+    xs = [normal(30 + s, t, 128, dtype=BF16) for s in range(4)]
+    want = [gpu.moe(x, w) for x in xs]
+    static = xs[0].clone()
+    graphs = []
+    for _ in range(2):                                             # two graphs of the same weights
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ids, weights = gpu.moe_route(static, args["router"], 4)
+            out = gpu.moe(static, w)
+        graphs.append((g, out, ids))
+    for x, y in zip(xs, want):
+        static.copy_(x)
+        for g, _, _ in graphs:
+            g.replay()
+        gpu.moe(xs[1], w)
+        torch.cuda.synchronize()
+        for _, out, ids in graphs:
+            assert torch.equal(out, y) and torch.equal(ids, gpu.moe_route(x, args["router"], 4)[0])
+
+
+def test_refusals(gpu):
+    r = normal(1, 8, 64, dtype=BF16)
+    gate, up, down = normal(2, 8, 32, 64, dtype=BF16), normal(3, 8, 32, 64, dtype=BF16), normal(4, 8, 64, 32, dtype=BF16)
+    x = normal(5, 3, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="top_k"):
+        gpu.moe_route(x, r, 9)
+    with pytest.raises(ValueError, match="top_k"):
+        gpu.moe_route(x, r, 0)
+    with pytest.raises(ValueError, match="router"):
+        gpu.moe_route(x.float(), r, 2)
+    with pytest.raises(ValueError, match="hidden"):
+        gpu.moe_route(normal(1, 3, 40, dtype=BF16), normal(1, 8, 40, dtype=BF16), 2)
+    with pytest.raises(ValueError, match="1 to 1024"):
+        gpu.moe_route(x, normal(1, 1025, 64, dtype=BF16), 2)
+    with pytest.raises(ValueError, match="up must be"):
+        gpu.MoeWeights(r, gate, up[:, :, :32], down, 2)
+    with pytest.raises(ValueError, match="4-bit or all plain"):
+        gpu.MoeWeights(r, gate, up, gpu.mx4_quantize(down), 2)
+    with pytest.raises(ValueError, match="float32"):
+        gpu.MoeWeights(r, gate, up, down.float(), 2)
+    with pytest.raises(ValueError, match="shared gate must be"):
+        gpu.MoeWeights(r, gate, up, down, 2, shared=(gate[:1, :16], up[:1], down[:1]))
+    with pytest.raises(ValueError, match="without shared"):
+        gpu.MoeWeights(r, gate, up, down, 2, shared_router=r[0])
+    w = gpu.MoeWeights(r, gate, up, down, 2)
+    with pytest.raises(ValueError, match=r"\[\.\.\., 64\]"):
+        gpu.moe(x[:, :32], w)
+    with pytest.raises(RuntimeError, match="gradient"):
+        gpu.moe(x.requires_grad_(), w)

@@ -1,0 +1,346 @@
+// Microscaled 4-bit weights (OCP MX: E2M1 elements, blocks of 32 along k with one
+// E8M0 scale), gfx950: quantisation, reading back, the layout of a checkpoint's
+// codes, and the product with activation rows.
+//
+// A block's scale is 2^s, s = max(floor(log2 max|w|) - 2, -127), so the largest
+// magnitude lies in [4, 8) scales; an element is w / 2^s to the nearest of
+// 0, .5, 1, 1.5, 2, 3, 4, 6 (ties to the even code), 6 beyond. The hardware
+// conversion (v_cvt_scalef32_pk_fp4_f32) does just that for every finite input,
+// subnormals included, so the division is exact. A block that holds a NaN or an
+// infinity becomes NaN as a whole (scale byte 255). A block of zeros has scale
+// byte 0.
+//
+// Weights are kept in the operand order of wtile.h, 17 bytes for 32 weights.
+#include "qwen4mix_internal.h"
+#include "wtile.h"
+
+namespace {
+
+constexpr int MX_NT = 256;
+
+struct MxGeom {
+  int n, k;          // a matrix
+  int rt, kt;        // its tiles
+  long tiles;        // of all matrices
+};
+
+MxGeom mx_geom(int mats, int n, int k) {
+  MxGeom g = {n, k, wt_row_tiles(n), wt_k_tiles(k), 0};
+  g.tiles = (long)mats * g.rt * g.kt;
+  return g;
+}
+
+// where a lane's block lies: its matrix row (of all matrices) and first column
+__device__ __forceinline__ bool block_of(const MxGeom& g, long tile, int lane, long& row, int& k0) {
+  const int ks = (int)(tile % g.kt);
+  const long rest = tile / g.kt;
+  const int r = (int)(rest % g.rt) * WT_ROWS + (lane & 15);
+  k0 = ks * WT_K + (lane >> 4) * MX_BLOCK;
+  row = rest / g.rt * g.n + r;
+  return r < g.n && k0 < g.k;
+}
+
+__device__ __forceinline__ void load32(const float* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 u = *reinterpret_cast<const float4*>(p + 4 * i);
+    v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+  }
+}
+__device__ __forceinline__ void load32(const bf16_t* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p + 8 * i);
+    const unsigned d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[8 * i + 2 * j] = __uint_as_float(d[j] << 16);
+      v[8 * i + 2 * j + 1] = __uint_as_float(d[j] & 0xffff0000u);
+    }
+  }
+}
+
+// one wave per tile, one lane per block
+template <typename T>
+__global__ __launch_bounds__(MX_NT) void mx4_quantize_kernel(MxGeom g, const T* w, uint8_t* codes, uint8_t* scales) {
+  const int lane = threadIdx.x & 63;
+  const long tile = (long)blockIdx.x * (MX_NT / 64) + (threadIdx.x >> 6);
+  if (tile >= g.tiles) return;
+  long row;
+  int k0;
+  u32x4_t q = {0u, 0u, 0u, 0u};
+  unsigned s = 0;
+  if (block_of(g, tile, lane, row, k0)) {
+    float v[32];
+    load32(w + row * g.k + k0, v);
+    unsigned amax = 0;                                     // magnitudes order as their bits do, NaN above all
+#pragma unroll
+    for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    if (amax >= 0x7f800000u) {
+      s = 255u;
+    } else {
+      s = (unsigned)max((int)(amax >> 23) - 2, 0);
+      const float scale = __uint_as_float(s << 23);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        unsigned c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * d], v[8 * d + 1], scale, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * d + 2], v[8 * d + 3], scale, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * d + 4], v[8 * d + 5], scale, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * d + 6], v[8 * d + 7], scale, 3);
+        q[d] = c;
+      }
+    }
+  }
+  *reinterpret_cast<u32x4_t*>(codes + tile * 1024 + lane * 16) = q;
+  scales[tile * 64 + lane] = (uint8_t)s;
+}
+
+__device__ __forceinline__ void store32(bf16_t* p, const u32x4_t& q, float scale) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    *reinterpret_cast<uint4*>(p + 8 * d) = __builtin_bit_cast(uint4, mx4_frag(q[d], scale));
+}
+__device__ __forceinline__ void store32(float* p, const u32x4_t& q, float scale) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 0);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 1);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 2);
+    const auto e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 3);
+    *reinterpret_cast<float4*>(p + 8 * d) = make_float4(a[0], a[1], b[0], b[1]);
+    *reinterpret_cast<float4*>(p + 8 * d + 4) = make_float4(c[0], c[1], e[0], e[1]);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(MX_NT) void mx4_dequantize_kernel(MxGeom g, const uint8_t* codes, const uint8_t* scales,
+                                                              T* out) {
+  const int lane = threadIdx.x & 63;
+  const long tile = (long)blockIdx.x * (MX_NT / 64) + (threadIdx.x >> 6);
+  if (tile >= g.tiles) return;
+  long row;
+  int k0;
+  if (!block_of(g, tile, lane, row, k0)) return;
+  const u32x4_t q = *reinterpret_cast<const u32x4_t*>(codes + tile * 1024 + lane * 16);
+  store32(out + row * g.k + k0, q, __uint_as_float((unsigned)scales[tile * 64 + lane] << 23));
+}
+
+// between the plain order (codes [rows, k / 2], scales [rows, k / 32]) and tiles
+template <bool TO_TILES>
+__global__ __launch_bounds__(MX_NT) void mx4_layout_kernel(MxGeom g, uint8_t* codes, uint8_t* scales, uint8_t* plain_codes,
+                                                          uint8_t* plain_scales) {
+  const int lane = threadIdx.x & 63;
+  const long tile = (long)blockIdx.x * (MX_NT / 64) + (threadIdx.x >> 6);
+  if (tile >= g.tiles) return;
+  long row;
+  int k0;
+  const bool in = block_of(g, tile, lane, row, k0);
+  uint4* tc = reinterpret_cast<uint4*>(codes + tile * 1024 + lane * 16);
+  uint8_t* ts = scales + tile * 64 + lane;
+  const long b = in ? row * (g.k / MX_BLOCK) + k0 / MX_BLOCK : 0;
+  if constexpr (TO_TILES) {
+    *tc = in ? *reinterpret_cast<const uint4*>(plain_codes + b * 16) : make_uint4(0u, 0u, 0u, 0u);
+    *ts = in ? plain_scales[b] : (uint8_t)0;
+  } else if (in) {
+    *reinterpret_cast<uint4*>(plain_codes + b * 16) = *tc;
+    plain_scales[b] = *ts;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// y[m][n] = sum_k W[n][k] x[m][k] for a few activation rows: a stream over the
+// weights. A workgroup takes TN row tiles against MT tiles of 16 activation
+// rows, its waves split the k tiles (PS of them in flight at a time), the partial
+// results meet in LDS. Every weight is loaded once per 16 MT rows.
+template <typename T>
+struct Mx4LinearArgs {
+  WMat w;
+  const T* x;
+  long ldx;
+  int m, n, k, rt, kt;
+  int n_seg;
+  int seg_end[QM_GEMV_MAX_SEG];
+  T* seg_out[QM_GEMV_MAX_SEG];
+};
+
+template <typename T, int TN, int MT, int NW, int PS>
+__global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4LinearArgs<T> A) {
+  using F = Fmt<WMx4, T>;
+  __shared__ f32x4_t s_red[NW][TN * MT][64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int g4 = lane >> 4, r16 = lane & 15;
+  const int t0 = blockIdx.x * TN, m0 = blockIdx.y * 16 * MT;
+  f32x4_t acc[TN][MT];
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) acc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wid; k0 < A.kt; k0 += NW * PS) {
+    typename F::W w[PS][TN];
+    typename F::X x[PS][MT];
+#pragma unroll
+    for (int p = 0; p < PS; ++p) {
+      const int ks = min(k0 + p * NW, A.kt - 1);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) w[p][t] = F::load_w(A.w, (long)min(t0 + t, A.rt - 1) * A.kt + ks, lane);
+      const int kb = ks * WT_K + g4 * MX_BLOCK;
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+        x[p][u] = F::load_x(kb < A.k ? A.x + (long)min(m0 + 16 * u + r16, A.m - 1) * A.ldx + kb : nullptr);
+    }
+#pragma unroll
+    for (int p = 0; p < PS; ++p)
+      if (k0 + p * NW < A.kt) F::step(acc, w[p], x[p]);
+  }
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) s_red[wid][t * MT + u][lane] = acc[t][u];
+  __syncthreads();
+  for (int r = wid; r < TN * MT; r += NW) {
+    f32x4_t v = s_red[0][r][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += s_red[w][r][lane];
+    const int n = (t0 + r / MT) * 16 + 4 * g4, m = m0 + 16 * (r % MT) + r16;
+    if (m >= A.m) continue;
+    int s = 0, start = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= A.n) break;
+      while (s + 1 < A.n_seg && n + i >= A.seg_end[s]) { start = A.seg_end[s]; ++s; }
+      Act<T>::store(A.seg_out[s], (long)m * (A.seg_end[s] - start) + (n + i - start), v[i]);
+    }
+  }
+}
+
+template <typename T, int TN, int MT, int NW, int PS>
+int launch_rows(const Mx4LinearArgs<T>& A, hipStream_t stream) {
+  hipLaunchKernelGGL((mx4_rows_kernel<T, TN, MT, NW, PS>),
+                     dim3((A.rt + TN - 1) / TN, (A.m + 16 * MT - 1) / (16 * MT)), dim3(64 * NW), 0, stream, A);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+template <typename T>
+int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
+  if (A.m <= 16) return launch_rows<T, 1, 1, 8, 2>(A, stream);
+  return launch_rows<T, 2, 2, 8, 1>(A, stream);
+}
+
+bool mx_sizes_ok(int mats, int n, int k) {
+  return mats > 0 && n > 0 && k > 0 && k % MX_BLOCK == 0 && n <= (1 << 24) && k <= (1 << 20);
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// grid of one wave per tile; 0 when the launch would be too large
+unsigned tile_grid(const MxGeom& g) {
+  const long nb = (g.tiles + MX_NT / 64 - 1) / (MX_NT / 64);
+  return nb > 0x7fffffffL / MX_NT ? 0u : (unsigned)nb;
+}
+
+}  // namespace
+
+extern "C" size_t qm_mx4_code_bytes(int mats, int n, int k) {
+  return mx_sizes_ok(mats, n, k) ? (size_t)mx_geom(mats, n, k).tiles * 1024 : 0;
+}
+
+#define QM_MX4_GEOM(name)                                                                                        \
+  if (!mx_sizes_ok(mats, n, k))                                                                                  \
+    return qm_fail(QM_ERR_ARG, name ": mats and n must be positive, k a positive multiple of 32 (n <= 2^24, k <= 2^20)"); \
+  const MxGeom g = mx_geom(mats, n, k);                                                                          \
+  const unsigned nb = tile_grid(g);                                                                              \
+  if (!nb) return qm_fail(QM_ERR_UNSUPPORTED, name ": too many tiles for one launch")
+
+extern "C" int qm_mx4_quantize(int act_dtype, int mats, int n, int k, const void* w, void* codes, void* scales,
+                               hipStream_t stream) {
+  if (act_dtype != QM_ACT_BF16 && act_dtype != QM_ACT_F32)
+    return qm_fail(QM_ERR_DTYPE, "qm_mx4_quantize: act_dtype must be QM_ACT_F32 or QM_ACT_BF16");
+  QM_MX4_GEOM("qm_mx4_quantize");
+  if (!w || !codes || !scales) return qm_fail(QM_ERR_ARG, "qm_mx4_quantize: null pointer");
+  if (!aligned16(w) || !aligned16(codes)) return qm_fail(QM_ERR_ARG, "qm_mx4_quantize: w and codes must be 16-byte aligned");
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+  if (act_dtype == QM_ACT_BF16)
+    hipLaunchKernelGGL(mx4_quantize_kernel<bf16_t>, dim3(nb), dim3(MX_NT), 0, stream, g, static_cast<const bf16_t*>(w), c, s);
+  else
+    hipLaunchKernelGGL(mx4_quantize_kernel<float>, dim3(nb), dim3(MX_NT), 0, stream, g, static_cast<const float*>(w), c, s);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+extern "C" int qm_mx4_dequantize(int act_dtype, int mats, int n, int k, const void* codes, const void* scales, void* w,
+                                 hipStream_t stream) {
+  if (act_dtype != QM_ACT_BF16 && act_dtype != QM_ACT_F32)
+    return qm_fail(QM_ERR_DTYPE, "qm_mx4_dequantize: act_dtype must be QM_ACT_F32 or QM_ACT_BF16");
+  QM_MX4_GEOM("qm_mx4_dequantize");
+  if (!w || !codes || !scales) return qm_fail(QM_ERR_ARG, "qm_mx4_dequantize: null pointer");
+  if (!aligned16(w) || !aligned16(codes))
+    return qm_fail(QM_ERR_ARG, "qm_mx4_dequantize: w and codes must be 16-byte aligned");
+  const uint8_t* c = static_cast<const uint8_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(scales);
+  if (act_dtype == QM_ACT_BF16)
+    hipLaunchKernelGGL(mx4_dequantize_kernel<bf16_t>, dim3(nb), dim3(MX_NT), 0, stream, g, c, s, static_cast<bf16_t*>(w));
+  else
+    hipLaunchKernelGGL(mx4_dequantize_kernel<float>, dim3(nb), dim3(MX_NT), 0, stream, g, c, s, static_cast<float*>(w));
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+extern "C" int qm_mx4_layout(int to_tiles, int mats, int n, int k, void* codes, void* scales, void* plain_codes,
+                             void* plain_scales, hipStream_t stream) {
+  QM_MX4_GEOM("qm_mx4_layout");
+  if (!codes || !scales || !plain_codes || !plain_scales) return qm_fail(QM_ERR_ARG, "qm_mx4_layout: null pointer");
+  if (!aligned16(codes) || !aligned16(plain_codes))
+    return qm_fail(QM_ERR_ARG, "qm_mx4_layout: codes must be 16-byte aligned");
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+  uint8_t* pc = static_cast<uint8_t*>(plain_codes);
+  uint8_t* ps = static_cast<uint8_t*>(plain_scales);
+  if (to_tiles)
+    hipLaunchKernelGGL(mx4_layout_kernel<true>, dim3(nb), dim3(MX_NT), 0, stream, g, c, s, pc, ps);
+  else
+    hipLaunchKernelGGL(mx4_layout_kernel<false>, dim3(nb), dim3(MX_NT), 0, stream, g, c, s, pc, ps);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+namespace {
+
+template <typename T>
+int linear(int m, int n, int k, const void* codes, const void* scales, const void* x, long ldx, int n_seg,
+           const int* seg_rows, void* const* seg_out, hipStream_t stream) {
+  Mx4LinearArgs<T> A = {};
+  A.w = {codes, static_cast<const uint8_t*>(scales)};
+  A.x = static_cast<const T*>(x);
+  A.ldx = ldx; A.m = m; A.n = n; A.k = k; A.rt = wt_row_tiles(n); A.kt = wt_k_tiles(k);
+  A.n_seg = n_seg;
+  long end = 0;
+  for (int s = 0; s < n_seg; ++s) {
+    end += seg_rows[s];
+    A.seg_end[s] = (int)end;
+    A.seg_out[s] = static_cast<T*>(seg_out[s]);
+  }
+  if (end != n) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: segment rows must add up to n");
+  return run_linear<T>(A, stream);
+}
+
+}  // namespace
+
+extern "C" int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* codes, const void* scales, const void* x,
+                             long ldx, int n_seg, const int* seg_rows, void* const* seg_out, hipStream_t stream) {
+  if (act_dtype != QM_ACT_BF16 && act_dtype != QM_ACT_F32)
+    return qm_fail(QM_ERR_DTYPE, "qm_mx4_linear: act_dtype must be QM_ACT_F32 or QM_ACT_BF16");
+  if (m <= 0 || m > 16 * 65535 || !mx_sizes_ok(1, n, k))
+    return qm_fail(QM_ERR_ARG, "qm_mx4_linear: m and n must be positive (m <= 1048560), k a positive multiple of 32");
+  if (!codes || !scales || !x || !seg_rows || !seg_out) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: null pointer");
+  const int unit = act_dtype == QM_ACT_BF16 ? 8 : 4;
+  if (ldx < k || ldx % unit) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: ldx must be at least k and whole 16-byte units");
+  if (!aligned16(codes) || !aligned16(x)) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: codes and x must be 16-byte aligned");
+  if (n_seg <= 0 || n_seg > QM_GEMV_MAX_SEG) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: 1..8 output segments");
+  for (int s = 0; s < n_seg; ++s)
+    if (seg_rows[s] <= 0 || !seg_out[s]) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: empty segment or null output");
+  if (act_dtype == QM_ACT_BF16)
+    return linear<bf16_t>(m, n, k, codes, scales, x, ldx, n_seg, seg_rows, seg_out, stream);
+  return linear<float>(m, n, k, codes, scales, x, ldx, n_seg, seg_rows, seg_out, stream);
+}

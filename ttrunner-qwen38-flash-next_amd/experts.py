@@ -1,0 +1,181 @@
+"""The mixture-of-experts layer: routing and the chosen experts' gated FFN.
+
+``moe_route`` picks each token's experts, ``moe`` is the whole layer over a
+``MoeWeights`` (reference/model.py:387-417): router, the chosen experts, and the
+shared experts that every token takes. ``Qwen4MixModel._moe`` builds the weights
+of a layer from the model's store, ``MixDecoder(ffn=True)`` runs it inside a
+decode step.
+
+Everything runs in the HIP kernels of libqwen4mix.so on the current stream of
+the tensors' device. Nothing here is differentiable.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, on_device
+
+MAX_EXPERTS, MAX_TOP_K, MAX_SHARED = 1024, 32, 32
+
+
+def _check_router(x: torch.Tensor, router: torch.Tensor, top_k: int) -> None:
+    experts, hidden = router.shape
+    if x.dim() < 1 or x.shape[-1] != hidden:
+        raise ValueError(f"x must be [..., {hidden}], got {tuple(x.shape)}")
+    if x.dtype != router.dtype or x.device != router.device:
+        raise ValueError(f"x is {x.dtype} on {x.device}, the router {router.dtype} on {router.device}")
+    if not 1 <= top_k <= min(experts, MAX_TOP_K):
+        raise ValueError(f"top_k must be 1 to {min(experts, MAX_TOP_K)}, got {top_k}")
+
+
+def _check_router_shape(router: torch.Tensor) -> None:
+    check_input(router, "the router")
+    if router.dim() != 2 or not 1 <= router.shape[0] <= MAX_EXPERTS:
+        raise ValueError(f"the router must be [experts, hidden] with 1 to {MAX_EXPERTS} experts, got "
+                         f"{tuple(router.shape)}")
+    if router.shape[1] == 0 or router.shape[1] % BLOCK:
+        raise ValueError(f"hidden must be a multiple of {BLOCK}, got {router.shape[1]}")
+
+
+def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool = True):
+    """The experts of each token: x [..., hidden], router [experts, hidden] (one
+    type, float32 or bfloat16) -> (ids int32 [..., top_k], weights float32
+    [..., top_k]).
+
+    ids are the experts of the largest logits x router^T in falling order (equal
+    ones: the lower index first; NaN above every number), weights their softmax
+    over all experts, or over the chosen ones when ``normalize``. The logits are
+    summed in float64, so that a token's experts do not depend on the rows beside
+    it."""
+    check_input(x, "x")
+    _check_router_shape(router)
+    _check_router(x, router, top_k)
+    experts, hidden = router.shape
+    ids = torch.empty(*x.shape[:-1], top_k, dtype=torch.int32, device=x.device)
+    weights = torch.empty(*x.shape[:-1], top_k, dtype=torch.float32, device=x.device)
+    m = x.numel() // hidden
+    if m:
+        xr, ldx = activation_rows(x)
+        rc = dense(router)
+        nbytes = native.load().qm_moe_route_workspace(m, experts)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        with on_device(x.device):
+            native.call("qm_moe_route", native.act_code(x.dtype), m, hidden, experts, top_k, int(bool(normalize)),
+                        native.ptr(xr), ldx, native.ptr(rc), native.ptr(ids), native.ptr(weights), native.ptr(ws),
+                        nbytes, native.stream_handle(x.device))
+    return ids, weights
+
+
+class _Tiles:
+    """A weight [mats, n, k] of the activations' type in the kernels' tile order."""
+
+    def __init__(self, w: torch.Tensor):
+        mats, n, k = w.shape
+        self.shape = w.shape
+        wc = dense(w)
+        tiles = -(-n // 16) * -(-k // 128)
+        self.codes = torch.empty(mats * tiles * 2048, dtype=w.dtype, device=w.device)
+        self.scales = None
+        with on_device(w.device):
+            native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), native.ptr(self.codes),
+                        native.stream_handle(w.device))
+
+
+class MoeWeights:
+    """The weights of a mixture-of-experts layer, laid out once for the kernels.
+
+    ``router`` [experts, hidden] sets the activations' type; ``gate``, ``up``
+    [experts, inter, hidden] and ``down`` [experts, hidden, inter] are tensors of
+    that type or ``Mx4Weight``s, and so is ``shared``, the (gate, up, down) of the
+    experts that every token takes (leading dimension: how many, each as wide as
+    a routed one), behind the sigmoid of ``shared_router`` [hidden] when that is
+    given. ``normalize``: a token's routed weights add up to 1."""
+
+    def __init__(self, router, gate, up, down, top_k: int, shared=None, shared_router=None, normalize: bool = True):
+        _check_router_shape(router)
+        self.router = dense(router.detach())
+        self.experts, self.hidden = router.shape
+        self.top_k, self.normalize = int(top_k), bool(normalize)
+        if not 1 <= self.top_k <= min(self.experts, MAX_TOP_K):
+            raise ValueError(f"top_k must be 1 to {min(self.experts, MAX_TOP_K)}, got {top_k}")
+        self.is_mx4 = isinstance(gate, Mx4Weight)
+        if len(gate.shape) != 3:
+            raise ValueError(f"gate must be [experts, inter, hidden], got {tuple(gate.shape)}")
+        self.inter = int(gate.shape[1])
+        if self.inter == 0 or self.inter % BLOCK:
+            raise ValueError(f"the experts' width must be a multiple of {BLOCK}, got {self.inter}")
+        self.gate, self.up, self.down = self._take(self.experts, (gate, up, down), "")
+        self.shared = 0
+        self.s_gate = self.s_up = self.s_down = self.shared_router = None
+        if shared is not None:
+            self.shared = int(shared[0].shape[0])
+            if not 1 <= self.shared <= MAX_SHARED:
+                raise ValueError(f"1 to {MAX_SHARED} shared experts, got {self.shared}")
+            self.s_gate, self.s_up, self.s_down = self._take(self.shared, shared, "shared ")
+            if shared_router is not None:
+                check_input(shared_router, "shared_router")
+                if shared_router.numel() != self.hidden or shared_router.dtype != router.dtype \
+                        or shared_router.device != router.device:
+                    raise ValueError(f"shared_router must be [{self.hidden}] in {router.dtype} on {router.device}")
+                self.shared_router = dense(shared_router.detach().reshape(-1))
+        elif shared_router is not None:
+            raise ValueError("shared_router without shared experts")
+        mats = (self.gate, self.up, self.down, self.s_gate, self.s_up, self.s_down)
+        p = [None if t is None else t.codes.data_ptr() for t in mats]
+        s = [None if t is None or t.scales is None else t.scales.data_ptr() for t in mats]
+        self._ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
+                                          native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
+
+    def _take(self, mats: int, parts, what: str) -> list:
+        out = []
+        for name, t, shape in zip(("gate", "up", "down"), parts, ((mats, self.inter, self.hidden),
+                                  (mats, self.inter, self.hidden), (mats, self.hidden, self.inter))):
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{what}{name} must be {shape}, got {tuple(t.shape)}")
+            if isinstance(t, Mx4Weight) != self.is_mx4:
+                raise ValueError("the experts' weights must all be 4-bit or all plain")
+            if t.device != self.router.device:
+                raise ValueError(f"{what}{name} is on {t.device}, the router on {self.router.device}")
+            if self.is_mx4:
+                out.append(t)
+                continue
+            check_input(t, what + name)
+            if t.dtype != self.router.dtype:
+                raise ValueError(f"{what}{name} is {t.dtype}, the router {self.router.dtype}")
+            out.append(_Tiles(t.detach()))
+        return out
+
+    @property
+    def dtype(self):
+        return self.router.dtype
+
+    @property
+    def device(self):
+        return self.router.device
+
+    def geom(self, rows: int) -> native.MoeGeom:
+        return native.MoeGeom(rows, self.hidden, self.inter, self.experts, self.shared, self.top_k,
+                              int(self.normalize), native.act_code(self.dtype),
+                              native.QM_W_MX4 if self.is_mx4 else native.QM_W_ACT)
+
+
+def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
+    """The layer's output for x [..., hidden] (the weights' type), in x's shape:
+    the weighted sum of each token's experts plus its shared experts."""
+    check_input(x, "x")
+    _check_router(x, weights.router, weights.top_k)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    m = x.numel() // weights.hidden
+    if m:
+        xr, ldx = activation_rows(x)
+        g = weights.geom(m)
+        nbytes = native.load().qm_moe_workspace(ctypes.byref(g))
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
+        with on_device(x.device):
+            native.call("qm_moe", ctypes.byref(g), ctypes.byref(weights._ptrs), native.ptr(xr), ldx, native.ptr(out),
+                        native.ptr(ws), nbytes, native.stream_handle(x.device))
+    return out

@@ -1,0 +1,181 @@
+"""Microscaled 4-bit weights and their products.
+
+A weight matrix in blocks of 32 along its last dimension: a block's elements are
+E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), its scale a power of two
+(E8M0), 17 bytes for 32 weights. ``mx4_quantize`` makes one from a float32 or
+bfloat16 tensor, ``Mx4Weight.from_codes`` from a checkpoint's codes, and
+``mx4_linear`` is ``F.linear`` over it for float32 or bfloat16 activations, from
+a single row to a prompt. ``Qwen4MixModel(weight_format="mx4")`` keeps a model's
+projections in it, ``MoeWeights`` a mixture-of-experts layer's.
+
+The weights live on the device in the matrix cores' operand order
+(include/qwen4mix.h); everything runs in the HIP kernels of libqwen4mix.so, on
+the current stream of the tensors' device. Nothing here is differentiable:
+inputs that require a gradient are refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from . import native
+
+BLOCK = 32
+TILE_ROWS, TILE_K = 16, 128
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one (launches go there)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def check_input(t: torch.Tensor, what: str) -> None:
+    """float32 or bfloat16 on the GPU, and nothing that would lose a gradient."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what} must be a tensor on the GPU")
+    native.act_code(t.dtype)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} requires a gradient, and this operator has none (use torch.no_grad())")
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy, contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def activation_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x [..., K] as rows [M, K] and the elements from one to the next: a view
+    where the kernels can read it (whole 16-byte units), else a copy."""
+    k = x.shape[-1]
+    rows = x.reshape(-1, k)
+    if rows.stride(1) == 1 and rows.data_ptr() % 16 == 0:
+        if rows.shape[0] == 1:
+            return rows, k
+        if rows.stride(0) >= k and rows.stride(0) * rows.element_size() % 16 == 0:
+            return rows, rows.stride(0)
+    return dense(rows), k
+
+
+class Mx4Weight:
+    """A weight [..., n, k] in 4-bit blocks along k, laid out for the kernels.
+
+    ``codes`` and ``scales`` are the device tiles; ``plain()`` gives them in a
+    checkpoint's order, ``dequantize()`` the values they stand for."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
+        self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def mats(self) -> int:
+        """Matrices in it (the product of the leading dimensions)."""
+        return self.shape[:-2].numel()
+
+    @staticmethod
+    def _check_shape(shape) -> None:
+        if len(shape) < 2 or 0 in shape:
+            raise ValueError(f"a 4-bit weight needs a non-empty [..., n, k], got {tuple(shape)}")
+        if shape[-1] % BLOCK:
+            raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {shape[-1]}")
+
+    @classmethod
+    def _empty(cls, shape, device) -> "Mx4Weight":
+        shape = torch.Size(shape)
+        cls._check_shape(shape)
+        nbytes = native.load().qm_mx4_code_bytes(shape[:-2].numel(), shape[-2], shape[-1])
+        if not nbytes:
+            raise ValueError(f"unsupported size of a 4-bit weight: {tuple(shape)}")
+        return cls(torch.empty(nbytes, dtype=torch.uint8, device=device),
+                   torch.empty(nbytes // 16, dtype=torch.uint8, device=device), shape)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mx4Weight":
+        """From codes uint8 [..., n, k / 2] (two elements a byte, the first in the
+        low nibble; bit 3 the sign, bits 2 and 1 the exponent, bit 0 the mantissa)
+        and scale bytes uint8 [..., n, k / 32] (2^(byte - 127), 255 NaN)."""
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda:
+            raise ValueError("codes and scales must be uint8 tensors on the GPU")
+        shape = codes.shape[:-1] + (2 * codes.shape[-1],)
+        cls._check_shape(shape)
+        if scales.shape != codes.shape[:-1] + (shape[-1] // BLOCK,) or scales.device != codes.device:
+            raise ValueError(f"scales must be {tuple(codes.shape[:-1]) + (shape[-1] // BLOCK,)} on {codes.device}, "
+                             f"got {tuple(scales.shape)} on {scales.device}")
+        w = cls._empty(shape, codes.device)
+        pc, ps = dense(codes), scales.contiguous()
+        with on_device(codes.device):
+            native.call("qm_mx4_layout", 1, w.mats, shape[-2], shape[-1], native.ptr(w.codes), native.ptr(w.scales),
+                        native.ptr(pc), native.ptr(ps), native.stream_handle(codes.device))
+        return w
+
+    def plain(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(codes, scales) in the order that ``from_codes`` takes."""
+        lead, n, k = self.shape[:-2], self.shape[-2], self.shape[-1]
+        codes = torch.empty(*lead, n, k // 2, dtype=torch.uint8, device=self.device)
+        scales = torch.empty(*lead, n, k // BLOCK, dtype=torch.uint8, device=self.device)
+        with on_device(self.device):
+            native.call("qm_mx4_layout", 0, self.mats, n, k, native.ptr(self.codes), native.ptr(self.scales),
+                        native.ptr(codes), native.ptr(scales), native.stream_handle(self.device))
+        return codes, scales
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, [..., n, k]: exact in float32 and in bfloat16 (a value past
+        their range is infinite)."""
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        with on_device(self.device):
+            native.call("qm_mx4_dequantize", native.act_code(dtype), self.mats, self.shape[-2], self.shape[-1],
+                        native.ptr(self.codes), native.ptr(self.scales), native.ptr(out),
+                        native.stream_handle(self.device))
+        return out
+
+
+def mx4_quantize(w: torch.Tensor) -> Mx4Weight:
+    """w [..., n, k] (float32 or bfloat16 on the GPU, k a multiple of 32) in
+    4-bit blocks: the scale 2^max(floor(log2 max|w|) - 2, -127), the elements to
+    the nearest value, ties to the even code, magnitudes above 6 scales to 6. A
+    block that holds a NaN or an infinity becomes NaN."""
+    check_input(w, "w")
+    out = Mx4Weight._empty(w.shape, w.device)
+    wc = dense(w)
+    with on_device(w.device):
+        native.call("qm_mx4_quantize", native.act_code(w.dtype), out.mats, w.shape[-2], w.shape[-1], native.ptr(wc),
+                    native.ptr(out.codes), native.ptr(out.scales), native.stream_handle(w.device))
+    return out
+
+
+def mx4_linear(x: torch.Tensor, weight: Mx4Weight, sections=None):
+    """F.linear(x, weight): x [..., k] -> [..., n] in x's type, summed in float.
+
+    ``sections``, a list of row counts that add up to n, splits the rows over
+    outputs of their own (the projections of one input kept as one weight): a
+    list of [..., rows] tensors is returned."""
+    check_input(x, "x")
+    if not isinstance(weight, Mx4Weight) or len(weight.shape) != 2:
+        raise ValueError("mx4_linear takes a 4-bit weight of one matrix [n, k]")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
+    if x.device != weight.device:
+        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
+    rows = [n] if sections is None else [int(r) for r in sections]
+    if min(rows, default=0) <= 0 or sum(rows) != n or len(rows) > 8:
+        raise ValueError(f"sections must be 1 to 8 positive row counts that add up to {n}, got {rows}")
+    outs = [torch.empty(*x.shape[:-1], r, dtype=x.dtype, device=x.device) for r in rows]
+    m = x.numel() // k
+    if m:
+        xr, ldx = activation_rows(x)
+        seg_rows = (ctypes.c_int * len(rows))(*rows)
+        seg_out = (ctypes.c_void_p * len(rows))(*[o.data_ptr() for o in outs])
+        with on_device(x.device):
+            native.call("qm_mx4_linear", native.act_code(x.dtype), m, n, k, native.ptr(weight.codes),
+                        native.ptr(weight.scales), native.ptr(xr), ldx, len(rows), seg_rows, seg_out,
+                        native.stream_handle(x.device))
+    return outs[0] if sections is None else outs

@@ -15,9 +15,12 @@ LIB_PATH = os.path.join(PKG, "libqwen4mix.so")
 
 QM_ACT_F32 = 0
 QM_ACT_BF16 = 1
+QM_W_ACT = 0
+QM_W_MX4 = 1
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_l = ctypes.c_long
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 
@@ -39,6 +42,17 @@ class QsaGeom(ctypes.Structure):
 
 class HcGeom(ctypes.Structure):
     _fields_ = [("rows", _i), ("streams", _i), ("hidden", _i), ("rank", _i), ("act_dtype", _i), ("eps", _f)]
+
+
+class MoeGeom(ctypes.Structure):
+    _fields_ = [(n, _i) for n in ("rows", "hidden", "inter", "experts", "shared", "top_k", "normalize", "act_dtype",
+                                  "weight_format")]
+
+
+class MoeWeightPtrs(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("router", "gate", "up", "down", "gate_scales", "up_scales", "down_scales",
+                                   "shared_router", "shared_gate", "shared_up", "shared_down", "shared_gate_scales",
+                                   "shared_up_scales", "shared_down_scales")]
 
 
 # name -> (restype, argtypes); every symbol include/qwen4mix.h declares
@@ -88,6 +102,16 @@ SIGNATURES = {
     "qm_hc_mix_as": (_i, [ctypes.POINTER(HcGeom), _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "qm_hc_mix": (_i, [ctypes.POINTER(HcGeom), _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "qm_hc_reinject": (_i, [ctypes.POINTER(HcGeom), _vp, _vp, _vp, _vp, _vp]),
+    "qm_mx4_code_bytes": (_sz, [_i, _i, _i]),
+    "qm_mx4_quantize": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "qm_mx4_dequantize": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "qm_mx4_layout": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "qm_mx4_linear": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _l, _i, _vp, _vp, _vp]),
+    "qm_moe_route_workspace": (_sz, [_i, _i]),
+    "qm_moe_route": (_i, [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "qm_tile_weight": (_i, [_i, _i, _i, _i, _vp, _vp, _vp]),
+    "qm_moe_workspace": (_sz, [ctypes.POINTER(MoeGeom)]),
+    "qm_moe": (_i, [ctypes.POINTER(MoeGeom), ctypes.POINTER(MoeWeightPtrs), _vp, _l, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None
