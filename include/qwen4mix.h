@@ -528,9 +528,9 @@ int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, in
                  hipStream_t stream);
 
 /* bf16 or float weights [mats, n, k] (row-major) into tiles of 16 rows x 128 k,
- * [mats][ceil(n/16)][ceil(k/128)], zeros past n and k: slot l of a tile holds k
- * 32 (l / 16) .. + 31 of row l % 16, its 16-byte pieces 1024 bytes apart (4 of
- * bf16, 8 of float). Both 16-byte aligned, k a multiple of 32. */
+ * [mats][ceil(n/16)][ceil(k/128)], zeros past n and k: pieces [4] of 64 slots,
+ * slot l of piece s holding k 32 s + 8 (l / 16) .. + 7 of row l % 16 (float: the
+ * two 16-byte halves 1024 bytes apart). Both 16-byte aligned, k a multiple of 32. */
 int qm_tile_weight(int act_dtype, int mats, int n, int k, const void* w, void* tiles, hipStream_t stream);
 
 typedef struct qm_moe_geom {

@@ -53,6 +53,25 @@ template <> struct Act<bf16_t> {
   __device__ __forceinline__ static float round(float v) { return bf16_to_f32(f32_to_bf16(v)); }
 };
 
+// 4 consecutive activations as float, and back
+__device__ __forceinline__ void load_act4(const bf16_t* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
+  v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load_act4(const float* p, float (&v)[4]) {
+  const float4 u = *reinterpret_cast<const float4*>(p);
+  v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+}
+template <typename V>
+__device__ __forceinline__ void store_act4(bf16_t* p, const V& v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+template <typename V>
+__device__ __forceinline__ void store_act4(float* p, const V& v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // A uniform value read through the constant address space, which the compiler
 // serves with a scalar load (for buffers the launch does not write, or words
 // it writes only after the read).

@@ -1,185 +1,20 @@
-// Mixture-of-experts layer, gfx950: the routing of token rows to experts and the
-// chosen experts' gated FFN (reference/model.py:387-417).
+// Mixture-of-experts layer, gfx950: the chosen experts' gated FFN
+// (reference/model.py:387-417), routed as route.hip does.
 //
-//   l[t][e] = sum_k x[t][k] R[e][k]            ids[t] = the top_k largest, ties to the lower index
-//   w[t][j] = softmax(l[t])[ids[t][j]]         (over the chosen ones alone when normalize)
-//   y[t]    = sum_j w[t][j] D_e (silu(G_e x[t]) * (U_e x[t]))
+//   y[t]    = sum_j w[t][j] D_e (silu(G_e x[t]) * (U_e x[t])),   e = ids[t][j]
 //           + sigmoid(x[t] . r) sum_s (shared expert s of x[t])
-//
-// Logits are sums of exact products in double: which experts a token takes then
-// depends on its values alone, not on the number of rows beside it or the order
-// of a sum, so a verify step routes as the single steps do.
 //
 // A pair is a (token, expert) choice; pair (top_k + shared) t + j is choice j of
 // token t, the shared experts its last ones. The pair's weight multiplies the
 // hidden row in float before that is rounded to the activations' type (the
 // operand of the second product), so the second products add up unweighted, in
 // the order of j.
-#include <stdio.h>
-
-#include "qwen4mix_internal.h"
-#include "wtile.h"
+#include "moe_internal.h"
+#include "moe_topk.h"
+#include "rows_mma.h"
+#include "wgemm.h"
 
 namespace {
-
-constexpr int RT_TB = 4;                 // token rows of one wave of the logits
-constexpr int RT_MAX_EXPERTS = 1024;
-constexpr int RT_MAX_TOPK = 32;
-
-template <typename T> struct Unit;       // 16 bytes as floats
-template <> struct Unit<bf16_t> {
-  static constexpr int VE = 8;
-  __device__ __forceinline__ static void get(const uint4& c, float (&v)[8]) {
-    const unsigned d[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(d[i] << 16);
-      v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
-    }
-  }
-};
-template <> struct Unit<float> {
-  static constexpr int VE = 4;
-  __device__ __forceinline__ static void get(const uint4& c, float (&v)[4]) {
-    v[0] = __uint_as_float(c.x); v[1] = __uint_as_float(c.y); v[2] = __uint_as_float(c.z); v[3] = __uint_as_float(c.w);
-  }
-};
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
-// logits[t][r], r < experts rows of the router and, when shared_router is given,
-// one more row for it
-template <typename T>
-struct LogitArgs {
-  const T* x;
-  long ldx;
-  const T* router;
-  const T* shared_router;
-  double* logits;
-  int rows, hidden, experts, cols;
-};
-
-template <typename T>
-__global__ __launch_bounds__(256) void moe_logits_kernel(LogitArgs<T> A) {
-  constexpr int VE = Unit<T>::VE;
-  const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= A.cols) return;
-  const int t0 = blockIdx.y * RT_TB;
-  const T* w = r < A.experts ? A.router + (long)r * A.hidden : A.shared_router;
-  double acc[RT_TB];
-#pragma unroll
-  for (int i = 0; i < RT_TB; ++i) acc[i] = 0.0;
-  for (int u = lane; u < A.hidden / VE; u += 64) {
-    float wv[VE];
-    Unit<T>::get(*reinterpret_cast<const uint4*>(w + (long)u * VE), wv);
-#pragma unroll
-    for (int i = 0; i < RT_TB; ++i) {
-      float xv[VE];
-      Unit<T>::get(*reinterpret_cast<const uint4*>(A.x + (long)min(t0 + i, A.rows - 1) * A.ldx + (long)u * VE), xv);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[i] = fma((double)wv[e], (double)xv[e], acc[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < RT_TB; ++i) {
-    const double s = wave_sum_f64(acc[i]);
-    if (lane == 0 && t0 + i < A.rows) A.logits[(long)(t0 + i) * A.cols + r] = s;
-  }
-}
-
-// A logit as an integer of the same order: NaN above everything, +0 and -0 equal.
-__device__ __forceinline__ long long logit_key(double v) {
-  if (v != v) return 0x7fffffffffffffffLL;
-  const long long b = __double_as_longlong(v + 0.0);
-  return b < 0 ? b ^ 0x7fffffffffffffffLL : b;
-}
-
-// One wave per token: lane l holds logits l, l + 64, ...; each round takes the
-// largest of what is left, the lowest index among equals.
-__global__ __launch_bounds__(256) void moe_topk_kernel(const double* logits, int rows, int cols, int experts, int top_k,
-                                                       int normalize, int* ids, float* weights, int ld_w, int shared) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= rows) return;
-  constexpr int PER = RT_MAX_EXPERTS / 64;
-  constexpr long long GONE = (long long)0x8000000000000000ULL;
-  const double* l = logits + (long)t * cols;
-  long long key[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 64 * i;
-    key[i] = e < experts ? logit_key(l[e]) : GONE;
-  }
-  double top = 0.0;
-  float mine = 0.f;                      // lane j: choice j's weight before the division
-  int mine_id = 0;
-  for (int j = 0; j < top_k; ++j) {
-    long long best = GONE;
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > best) { best = key[i]; at = lane + 64 * i; }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      const long long ob = __shfl_xor(best, m, 64);
-      const int oa = __shfl_xor(at, m, 64);
-      if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 64 * i == at) key[i] = GONE;
-    const double v = l[at];
-    if (j == 0) top = v;
-    if (lane == j) { mine = expf((float)(v - top)); mine_id = at; }
-  }
-  float sum = 0.f;
-  if (normalize) {
-    sum = wave_sum(lane < top_k ? mine : 0.f);
-  } else {
-    for (int e = lane; e < experts; e += 64) sum += expf((float)(l[e] - top));
-    sum = wave_sum(sum);
-  }
-  if (lane < top_k) {
-    ids[(long)t * top_k + lane] = mine_id;
-    weights[(long)t * ld_w + lane] = mine / sum;
-  }
-  if (lane < shared) {
-    float g = 1.f;
-    if (cols > experts) g = (float)(1.0 / (1.0 + exp(-l[experts])));
-    weights[(long)t * ld_w + top_k + lane] = g;
-  }
-}
-
-// Each expert's pairs in the tokens' order (a workgroup per expert)
-__global__ __launch_bounds__(256) void moe_lists_kernel(const int* ids, int rows, int top_k, int ppt, int* counts,
-                                                        int* lists) {
-  __shared__ int s_wave[4];
-  const int e = blockIdx.x, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int n = rows * top_k;
-  int* list = lists + (long)e * rows;
-  int at = 0;
-  for (int p0 = 0; p0 < n; p0 += 256) {
-    const int p = p0 + threadIdx.x;
-    const bool hit = p < n && ids[p] == e;
-    const unsigned long long m = __builtin_amdgcn_ballot_w64(hit);
-    if (lane == 0) s_wave[wid] = __popcll(m);
-    __syncthreads();
-    int before = at, all = 0;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wid) before += s_wave[w];
-      all += s_wave[w];
-    }
-    if (hit) list[before + __popcll(m & ((1ull << lane) - 1ull))] = p / top_k * ppt + p % top_k;
-    at += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) counts[e] = at;
-}
 
 template <typename T>
 struct MoeArgs {
@@ -189,9 +24,11 @@ struct MoeArgs {
   WMat gate, up, down, s_gate, s_up, s_down;
   const int* counts;
   const int* lists;
+  const int* n_tiles;
+  const int2* tiles;   // row tiles of the many-row kernels
   const float* pair_w;
   T* h;              // [pairs][inter]
-  float* part;       // [pairs][hidden]
+  T* part;           // [pairs][hidden]
   T* out;            // [rows][hidden]
 };
 
@@ -215,200 +52,420 @@ __device__ __forceinline__ int pair_of(const ExpertRows& r, int i, int ppt) {
 __device__ __forceinline__ WMat expert_mat(const WMat& m, int e, long tiles, int tile_bytes) {
   return {static_cast<const char*>(m.data) + (long)e * tiles * tile_bytes, m.scales ? m.scales + (long)e * tiles * 64 : nullptr};
 }
-template <typename WF> __device__ __forceinline__ constexpr int tile_bytes() {
-  return sizeof(WF) && __is_same(WF, WMx4) ? 1024 : __is_same(WF, WBf16) ? 4096 : 8192;
-}
-
-// h = w silu(G x) (U x): a workgroup per (TN tiles of hidden units, expert), the
-// waves split k, 16 MT pairs at a time
-template <typename WF, typename T, int TN, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) void moe_up_kernel(MoeArgs<T> A) {
-  using F = Fmt<WF, T>;
-  __shared__ f32x4_t s_red[NW][2 * TN * MT][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int g4 = lane >> 4, r16 = lane & 15;
-  const ExpertRows R = expert_rows(A, blockIdx.y);
-  const int t0 = blockIdx.x * TN;
-  const int rt = wt_row_tiles(A.inter), kt = wt_k_tiles(A.hidden);
-  const WMat gate = expert_mat(R.is_shared ? A.s_gate : A.gate, R.e, (long)rt * kt, tile_bytes<WF>());
-  const WMat up = expert_mat(R.is_shared ? A.s_up : A.up, R.e, (long)rt * kt, tile_bytes<WF>());
-  for (int m0 = 0; m0 < R.count; m0 += 16 * MT) {
-    const T* xp[MT];
-#pragma unroll
-    for (int u = 0; u < MT; ++u)
-      xp[u] = A.x + (long)(pair_of(R, min(m0 + 16 * u + r16, R.count - 1), A.ppt) / A.ppt) * A.ldx;
-    f32x4_t acc[2 * TN][MT];
-#pragma unroll
-    for (int t = 0; t < 2 * TN; ++t)
-#pragma unroll
-      for (int u = 0; u < MT; ++u) acc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int ks = wid; ks < kt; ks += NW) {
-      typename F::W w[2 * TN];
-      typename F::X x[MT];
-#pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        const long tile = (long)min(t0 + t, rt - 1) * kt + ks;
-        w[t] = F::load_w(gate, tile, lane);
-        w[TN + t] = F::load_w(up, tile, lane);
-      }
-      const int kb = ks * WT_K + g4 * MX_BLOCK;
-#pragma unroll
-      for (int u = 0; u < MT; ++u) x[u] = F::load_x(kb < A.hidden ? xp[u] + kb : nullptr);
-      F::step(acc, w, x);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 2 * TN; ++t)
-#pragma unroll
-      for (int u = 0; u < MT; ++u) s_red[wid][t * MT + u][lane] = acc[t][u];
-    __syncthreads();
-    for (int r = wid; r < TN * MT; r += NW) {
-      f32x4_t a = s_red[0][r][lane], b = s_red[0][TN * MT + r][lane];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) {
-        a += s_red[w][r][lane];
-        b += s_red[w][TN * MT + r][lane];
-      }
-      const int n = (t0 + r / MT) * 16 + 4 * g4, m = m0 + 16 * (r % MT) + r16;
-      if (m < R.count && n < A.inter) {                      // inter is a multiple of 4
-        const int p = pair_of(R, m, A.ppt);
-        const float w = A.pair_w[p];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) Act<T>::store(A.h, (long)p * A.inter + n + i, w * (silu_f(a[i]) * b[i]));
-      }
-    }
-  }
-}
-
-// part[pair] = D h[pair]
-template <typename WF, typename T, int TN, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) void moe_down_kernel(MoeArgs<T> A) {
-  using F = Fmt<WF, T>;
-  __shared__ f32x4_t s_red[NW][TN * MT][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int g4 = lane >> 4, r16 = lane & 15;
-  const ExpertRows R = expert_rows(A, blockIdx.y);
-  const int t0 = blockIdx.x * TN;
-  const int rt = wt_row_tiles(A.hidden), kt = wt_k_tiles(A.inter);
-  const WMat down = expert_mat(R.is_shared ? A.s_down : A.down, R.e, (long)rt * kt, tile_bytes<WF>());
-  for (int m0 = 0; m0 < R.count; m0 += 16 * MT) {
-    const T* hp[MT];
-#pragma unroll
-    for (int u = 0; u < MT; ++u)
-      hp[u] = A.h + (long)pair_of(R, min(m0 + 16 * u + r16, R.count - 1), A.ppt) * A.inter;
-    f32x4_t acc[TN][MT];
-#pragma unroll
-    for (int t = 0; t < TN; ++t)
-#pragma unroll
-      for (int u = 0; u < MT; ++u) acc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int ks = wid; ks < kt; ks += NW) {
-      typename F::W w[TN];
-      typename F::X x[MT];
-#pragma unroll
-      for (int t = 0; t < TN; ++t) w[t] = F::load_w(down, (long)min(t0 + t, rt - 1) * kt + ks, lane);
-      const int kb = ks * WT_K + g4 * MX_BLOCK;
-#pragma unroll
-      for (int u = 0; u < MT; ++u) x[u] = F::load_x(kb < A.inter ? hp[u] + kb : nullptr);
-      F::step(acc, w, x);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < TN; ++t)
-#pragma unroll
-      for (int u = 0; u < MT; ++u) s_red[wid][t * MT + u][lane] = acc[t][u];
-    __syncthreads();
-    for (int r = wid; r < TN * MT; r += NW) {
-      f32x4_t a = s_red[0][r][lane];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) a += s_red[w][r][lane];
-      const int n = (t0 + r / MT) * 16 + 4 * g4, m = m0 + 16 * (r % MT) + r16;
-      if (m < R.count && n < A.hidden)
-        *reinterpret_cast<f32x4_t*>(A.part + (long)pair_of(R, m, A.ppt) * A.hidden + n) = a;
-    }
-  }
-}
+// ---------------------------------------------------------------------------
+// A few tokens (at most FEW): the logits, the up products and the down products,
+// three launches over the chosen experts' weights alone.
+//
+// An operand holds 16 activation rows: all tokens' rows stand in it, whichever
+// expert is multiplied, and a column counts where its token chose the expert. A
+// slot is a shared expert or one of the distinct chosen ones, in the order of
+// their numbers. A single token's workgroups rank its logits for themselves (a
+// launch of its own for that takes longer); for several tokens one workgroup
+// does and leaves the table of slots.
+// ---------------------------------------------------------------------------
+constexpr int FEW = 16;
+constexpr int FEW_UP_NW = 8, FEW_DOWN_NW = 16;
 
 template <typename T>
+struct FewArgs {
+  MoeArgs<T> m;
+  const double* logits;
+  int cols, normalize;
+  int* n_slots;        // of the table
+  int* slot_expert;    // [slot] expert; of a shared one -1 - its number
+  int* slot_pair;      // [slot][16] the pair of each column, -1 where none
+  float* slot_w;       // [slot][16] its weight
+};
+
+// choice `lane` of a token and its weight, by one wave
+template <int PER>
+__device__ __forceinline__ int wave_choose(const double* l, int experts, int top_k, int normalize, int lane, float& weight) {
+  WaveTop<PER> top;
+  top.load(l, experts, lane);
+  int id = 0;
+  double v = 0.0, v0 = 0.0;
+  for (int j = 0; j < top_k; ++j) {
+    long long best;
+    const int at = top.take(lane, best);
+    const double d = key_logit(best);
+    if (j == 0) v0 = d;
+    if (lane == j) { id = at; v = d; }
+  }
+  const float mine = lane < top_k ? expf((float)(v - v0)) : 0.f;
+  float sum = mine;
+  if (!normalize) {
+    sum = 0.f;
+    for (int i = lane; i < experts; i += 64) sum += expf((float)(l[i] - v0));
+  }
+  weight = mine / wave_sum(sum);
+  return id;
+}
+template <typename T> __device__ __forceinline__ float shared_weight(const FewArgs<T>& A, int t) {
+  return A.cols > A.m.experts ? sigmoid_f((float)A.logits[(long)t * A.cols + A.m.experts]) : 1.f;
+}
+
+// The table of slots, by one workgroup with a wave per token
+template <typename T, int PER>
+__global__ __launch_bounds__(64 * FEW) void moe_few_plan_kernel(FewArgs<T> A) {
+  __shared__ int s_ids[FEW][RT_MAX_TOPK];
+  __shared__ float s_w[FEW][RT_MAX_TOPK];
+  __shared__ unsigned s_map[RT_MAX_EXPERTS / 32];
+  __shared__ int s_before[RT_MAX_EXPERTS / 32 + 1];
+  const MoeArgs<T>& M = A.m;
+  const int lane = threadIdx.x & 63, t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x < RT_MAX_EXPERTS / 32) s_map[threadIdx.x] = 0u;
+  __syncthreads();
+  if (t < M.rows) {
+    float w;
+    const int id = wave_choose<PER>(A.logits + (long)t * A.cols, M.experts, M.top_k, A.normalize, lane, w);
+    if (lane < M.top_k) {
+      s_ids[t][lane] = id;
+      s_w[t][lane] = w;
+      atomicOr(&s_map[id >> 5], 1u << (id & 31));
+    }
+  }
+  // every column of every slot none, before the choices fill theirs
+  const int most = M.shared + min(M.rows * M.top_k, M.experts);
+  for (int i = threadIdx.x; i < most * 16; i += 64 * FEW) A.slot_pair[i] = -1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = M.shared;
+    for (int i = 0; i < RT_MAX_EXPERTS / 32; ++i) {
+      s_before[i] = n;
+      n += __popc(s_map[i]);
+    }
+    *A.n_slots = n;
+  }
+  __syncthreads();
+  if (t < M.rows && lane < M.top_k) {
+    const int e = s_ids[t][lane], slot = s_before[e >> 5] + __popc(s_map[e >> 5] & ((1u << (e & 31)) - 1u));
+    A.slot_expert[slot] = e;                                 // the same value from every token that chose it
+    A.slot_pair[slot * 16 + t] = t * M.ppt + lane;
+    A.slot_w[slot * 16 + t] = s_w[t][lane];
+  }
+  if (t < M.rows && lane < M.shared) {
+    A.slot_expert[lane] = -1 - lane;
+    A.slot_pair[lane * 16 + t] = t * M.ppt + M.top_k + lane;
+    A.slot_w[lane * 16 + t] = shared_weight(A, t);
+  }
+}
+
+// h of a slot: a workgroup per 16 hidden units and slot, the waves split k
+template <typename WF, typename T, int PER, bool ONE>
+__global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A) {
+  using F = Fmt<WF, T>;
+  constexpr int NW = FEW_UP_NW, KP = 2;                      // k tiles in flight
+  __shared__ f32x4_t s_red[NW][2][64];
+  __shared__ int s_id[RT_MAX_TOPK];
+  __shared__ float s_w[RT_MAX_TOPK];
+  const MoeArgs<T>& M = A.m;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g4 = lane >> 4, r16 = lane & 15;
+  const int kt = wt_k_tiles(M.hidden), rt = wt_row_tiles(M.inter), slot = blockIdx.y;
+  const T* row = M.x + (long)min(r16, M.rows - 1) * M.ldx;
+  Acts<F, T> pre[KP];                                        // before it is known which expert
+#pragma unroll
+  for (int p = 0; p < KP; ++p) pre[p].load(row, min(wid + p * NW, kt - 1), M.hidden, g4);
+  int e, pair = -1;
+  float weight = 0.f;
+  if constexpr (ONE) {
+    if (slot < M.shared) {
+      e = -1 - slot;
+      weight = shared_weight(A, 0);
+    } else {
+      if (wid == 0) {
+        float w;
+        const int id = wave_choose<PER>(A.logits, M.experts, M.top_k, A.normalize, lane, w);
+        if (lane < M.top_k) { s_id[lane] = id; s_w[lane] = w; }
+      }
+      __syncthreads();
+      e = __builtin_amdgcn_readfirstlane(s_id[slot - M.shared]);
+      weight = s_w[slot - M.shared];
+    }
+    if (r16 == 0) pair = slot < M.shared ? M.top_k + slot : slot - M.shared;
+    if (blockIdx.x == 0 && threadIdx.x < 16) {               // for the down products
+      A.slot_pair[slot * 16 + threadIdx.x] = pair;
+      if (threadIdx.x == 0) A.slot_expert[slot] = e;
+      if (threadIdx.x == 0 && slot == 0) *A.n_slots = gridDim.y;
+    }
+  } else {
+    if (slot >= *A.n_slots) return;
+    e = A.slot_expert[slot];
+    pair = A.slot_pair[slot * 16 + r16];
+    weight = A.slot_w[slot * 16 + r16];
+  }
+  const WMat gate = expert_mat(e < 0 ? M.s_gate : M.gate, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
+  const WMat up = expert_mat(e < 0 ? M.s_up : M.up, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
+  f32x4_t acc[2][1];
+  clear(acc);
+  for (int k0 = wid; k0 < kt; k0 += NW * KP) {
+    typename F::W w[KP][2];
+    Acts<F, T> x[KP][1];
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int ks = min(k0 + p * NW, kt - 1);
+      w[p][0] = F::load_w(gate, (long)blockIdx.x * kt + ks, lane);
+      w[p][1] = F::load_w(up, (long)blockIdx.x * kt + ks, lane);
+      if (k0 == wid) x[p][0] = pre[p];
+      else x[p][0].load(row, ks, M.hidden, g4);
+    }
+#pragma unroll
+    for (int p = 0; p < KP; ++p)
+      if (k0 + p * NW < kt) step_tile<F, T>(acc, w[p], x[p]);
+  }
+  s_red[wid][0][lane] = acc[0][0];
+  s_red[wid][1][lane] = acc[1][0];
+  __syncthreads();
+  if (wid != 0 || pair < 0) return;
+  f32x4_t a = s_red[0][0][lane], b = s_red[0][1][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    a += s_red[w][0][lane];
+    b += s_red[w][1][lane];
+  }
+  const int n = blockIdx.x * 16 + 4 * g4;
+  if (n >= M.inter) return;
+  f32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = weight * (silu_f(a[i]) * b[i]);
+  store_act4(M.h + (long)pair * M.inter + n, v);
+}
+
+// out: a workgroup per 16 outputs; the waves share the (slot, k tile) units
+template <typename WF, typename T>
+__global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<T> A) {
+  using F = Fmt<WF, T>;
+  constexpr int NW = FEW_DOWN_NW, U = 2;
+  __shared__ f32x4_t s_red[NW][64];
+  const MoeArgs<T>& M = A.m;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g4 = lane >> 4, r16 = lane & 15;
+  const int kt = wt_k_tiles(M.inter), rt = wt_row_tiles(M.hidden);
+  const int units = *A.n_slots * kt;
+  f32x4_t total = {0.f, 0.f, 0.f, 0.f};
+  for (int u0 = wid; u0 < units; u0 += NW * U) {
+    typename F::W w[U][1];
+    Acts<F, T> x[U][1];
+    int pair[U];
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      const int u = min(u0 + p * NW, units - 1), slot = u / kt, ks = u % kt;
+      const int e = A.slot_expert[slot];
+      pair[p] = A.slot_pair[slot * 16 + r16];
+      const WMat down = expert_mat(e < 0 ? M.s_down : M.down, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
+      w[p][0] = F::load_w(down, (long)blockIdx.x * kt + ks, lane);
+      x[p][0].load(M.h + (long)max(pair[p], 0) * M.inter, ks, M.inter, g4);
+    }
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      if (u0 + p * NW >= units) continue;
+      f32x4_t acc[1][1];
+      clear(acc);
+      step_tile<F, T>(acc, w[p], x[p]);
+      // a token that did not choose the expert takes nothing from it, whatever it is
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[i] += pair[p] < 0 ? 0.f : acc[0][0][i];
+    }
+  }
+  s_red[wid][lane] = total;
+  __syncthreads();
+  if (wid != 0 || r16 >= M.rows) return;
+  f32x4_t v = s_red[0][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v += s_red[w][lane];
+  const int n = blockIdx.x * 16 + 4 * g4;
+  if (n < M.hidden) store_act4(M.out + (long)r16 * M.hidden + n, v);
+}
+
+// ---------------------------------------------------------------------------
+// Many tokens: routing, the experts' lists of pairs, the up products, the down
+// products of every pair, and their sum per token.
+// ---------------------------------------------------------------------------
+// The same over many rows (wgemm.h): a workgroup per row tile of the table and
+// range of weight rows, the ranges of a tile side by side on an XCD. Of a wave's
+// TN row tiles the first half are gate rows, the others the up rows of the same
+// hidden units.
+template <typename WF, typename T, int TN, int TM, int WN, int WM, int S>
+__global__ __launch_bounds__(64 * WN * WM, 2) void moe_up_gemm_kernel(MoeArgs<T> A) {
+  using G = SpanGemm<WF, T, TN, TM, WN, WM, S>;
+  constexpr int HN = TN / 2;
+  extern __shared__ __attribute__((aligned(16))) char s_buf[];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rt = wt_row_tiles(A.inter), kt = wt_k_tiles(A.hidden);
+  const int nt = (rt + HN * WN - 1) / (HN * WN), items = *A.n_tiles * nt;
+  if ((int)blockIdx.x >= items) return;
+  const int item = xcd_run(blockIdx.x, items);
+  const int2 tile = A.tiles[item / nt];
+  const ExpertRows R = expert_rows(A, tile.x);
+  const int t0 = item % nt * WN * HN;
+  const WMat gate = expert_mat(R.is_shared ? A.s_gate : A.gate, R.e, (long)rt * kt, G::F::TILE);
+  const WMat up = expert_mat(R.is_shared ? A.s_up : A.up, R.e, (long)rt * kt, G::F::TILE);
+  auto first = [&](int q) { return (long)min(t0 + q / TN * HN + q % HN, rt - 1) * kt; };
+  const typename G::Src src = G::source(
+      wid, lane,
+      [&](int i) { return A.x + (long)(pair_of(R, min(tile.y + i, R.count - 1), A.ppt) / A.ppt) * A.ldx; },
+      [&](int q) { return static_cast<const char*>(q % TN < HN ? gate.data : up.data) + first(q) * G::F::TILE; },
+      [&](int q) { return (q % TN < HN ? gate.scales : up.scales) + first(q) * 64; });
+  f32x4_t acc[TN][TM];
+  clear(acc);
+  G::run(acc, s_buf, src, A.hidden);
+#pragma unroll
+  for (int u = 0; u < TM; ++u) {
+    const int m = tile.y + (wid % WM) * 16 * TM + 16 * u + (lane & 15);
+    if (m >= R.count) continue;
+    const int p = pair_of(R, m, A.ppt);
+    const float w = A.pair_w[p];
+#pragma unroll
+    for (int t = 0; t < HN; ++t) {
+      const int n = (t0 + wid / WM * HN + t) * 16 + 4 * (lane >> 4);
+      if (n >= A.inter) continue;
+      f32x4_t v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = w * (silu_f(acc[t][u][i]) * acc[HN + t][u][i]);
+      store_act4(A.h + (long)p * A.inter + n, v);
+    }
+  }
+}
+
+template <typename WF, typename T, int TN, int TM, int WN, int WM, int S>
+__global__ __launch_bounds__(64 * WN * WM, 2) void moe_down_gemm_kernel(MoeArgs<T> A) {
+  using G = SpanGemm<WF, T, TN, TM, WN, WM, S>;
+  extern __shared__ __attribute__((aligned(16))) char s_buf[];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rt = wt_row_tiles(A.hidden), kt = wt_k_tiles(A.inter);
+  const int nt = (rt + TN * WN - 1) / (TN * WN), items = *A.n_tiles * nt;
+  if ((int)blockIdx.x >= items) return;
+  const int item = xcd_run(blockIdx.x, items);
+  const int2 tile = A.tiles[item / nt];
+  const ExpertRows R = expert_rows(A, tile.x);
+  const int t0 = item % nt * WN * TN;
+  const WMat down = expert_mat(R.is_shared ? A.s_down : A.down, R.e, (long)rt * kt, G::F::TILE);
+  auto first = [&](int q) { return (long)min(t0 + q, rt - 1) * kt; };
+  const typename G::Src src = G::source(
+      wid, lane, [&](int i) { return A.h + (long)pair_of(R, min(tile.y + i, R.count - 1), A.ppt) * A.inter; },
+      [&](int q) { return static_cast<const char*>(down.data) + first(q) * G::F::TILE; },
+      [&](int q) { return down.scales + first(q) * 64; });
+  f32x4_t acc[TN][TM];
+  clear(acc);
+  G::run(acc, s_buf, src, A.inter);
+#pragma unroll
+  for (int u = 0; u < TM; ++u) {
+    const int m = tile.y + (wid % WM) * 16 * TM + 16 * u + (lane & 15);
+    if (m >= R.count) continue;
+    T* o = A.part + (long)pair_of(R, m, A.ppt) * A.hidden;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      const int n = (t0 + wid / WM * TN + t) * 16 + 4 * (lane >> 4);
+      if (n < A.hidden) store_act4(o + n, acc[t][u]);
+    }
+  }
+}
+
+// y[t] = the sum of its pairs' products, in their order (a thread per 16 bytes)
+template <typename T>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs<T> A) {
+  constexpr int VE = 16 / sizeof(T);
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int per = A.hidden / 4;
+  const int per = A.hidden / VE;
   if (i >= (long)A.rows * per) return;
   const long t = i / per;
-  const int c = (int)(i % per) * 4;
-  const float* p = A.part + t * A.ppt * A.hidden + c;
-  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < A.ppt; ++j) v += *reinterpret_cast<const f32x4_t*>(p + (long)j * A.hidden);
+  const int c = (int)(i % per) * VE;
+  const T* p = A.part + t * A.ppt * A.hidden + c;
+  float v[VE];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) Act<T>::store(A.out, t * A.hidden + c + e, v[e]);
+  for (int e = 0; e < VE; ++e) v[e] = 0.f;
+  for (int j = 0; j < A.ppt; ++j) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p + (long)j * A.hidden);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] += Chunk<T>::get(u, e);
+  }
+  *reinterpret_cast<uint4*>(A.out + t * A.hidden + c) = Chunk<T>::pack(v);
 }
 
 // rows of bf16 or float weights into tiles (a wave per tile)
 template <typename T>
 __global__ __launch_bounds__(256) void tile_weight_kernel(int n, int k, int rt, int kt, long tiles, const T* w, char* out) {
-  constexpr int VE = Unit<T>::VE, PIECES = 32 / VE;
+  constexpr int VE = 16 / sizeof(T), PIECES = 32 / VE;
   const int lane = threadIdx.x & 63;
   const long tile = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (tile >= tiles) return;
   const int ks = (int)(tile % kt);
   const long rest = tile / kt;
-  const int r = (int)(rest % rt) * WT_ROWS + (lane & 15), k0 = ks * WT_K + (lane >> 4) * MX_BLOCK;
-  const bool in = r < n && k0 < k;
-  const T* src = w + ((rest / rt) * n + r) * (long)k + k0;
+  const int r = (int)(rest % rt) * WT_ROWS + (lane & 15);
+  const T* src = w + ((rest / rt) * n + r) * (long)k;
   char* dst = out + tile * (PIECES * 1024) + lane * 16;
 #pragma unroll
-  for (int s = 0; s < PIECES; ++s)
+  for (int s = 0; s < PIECES; ++s) {
+    // piece s / HALVES of 8 k, its half s % HALVES
+    constexpr int HALVES = 8 / VE;
+    const int k0 = ks * WT_K + 32 * (s / HALVES) + 8 * (lane >> 4) + s % HALVES * VE;
     *reinterpret_cast<uint4*>(dst + s * 1024) =
-        in ? *reinterpret_cast<const uint4*>(src + s * VE) : make_uint4(0u, 0u, 0u, 0u);
+        r < n && k0 < k ? *reinterpret_cast<const uint4*>(src + k0) : make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T>
-int launch_logits(const LogitArgs<T>& A, hipStream_t stream) {
-  hipLaunchKernelGGL(moe_logits_kernel<T>, dim3((A.cols + 3) / 4, (A.rows + RT_TB - 1) / RT_TB), dim3(256), 0, stream, A);
-  QM_CHECK_LAUNCH();
-  return QM_OK;
-}
-
-int check_route(const char* what, int act_dtype, int rows, int hidden, int experts, int top_k, long ldx) {
-  static thread_local char msg[160];
-  const int unit = act_dtype == QM_ACT_BF16 ? 8 : 4;
-  const char* bad = nullptr;
-  int code = QM_ERR_ARG;
-  if (act_dtype != QM_ACT_BF16 && act_dtype != QM_ACT_F32) { bad = "act_dtype must be QM_ACT_F32 or QM_ACT_BF16"; code = QM_ERR_DTYPE; }
-  else if (rows <= 0 || rows > 4 * 65535) bad = "rows must be 1..262140";
-  else if (hidden <= 0 || hidden % 32 || hidden > (1 << 20)) bad = "hidden must be a positive multiple of 32 (at most 2^20)";
-  else if (experts <= 0 || experts > RT_MAX_EXPERTS) { bad = "experts must be 1..1024"; code = QM_ERR_UNSUPPORTED; }
-  else if (top_k <= 0 || top_k > RT_MAX_TOPK || top_k > experts) bad = "top_k must be 1..32 and at most experts";
-  else if (ldx < hidden || ldx % unit) bad = "ldx must be at least hidden and whole 16-byte units";
-  if (!bad) return QM_OK;
-  snprintf(msg, sizeof(msg), "%s: %s", what, bad);
-  return qm_fail(code, msg);
-}
-
 struct MoeLayout {
-  size_t logits, ids, pair_w, counts, lists, h, part, bytes;
+  size_t logits, norms, ids, pair_w, counts, lists, meta, tiles, h, part, bytes;
+  long max_tiles;      // of row tiles of bm rows
+  int bm;
 };
+
+// Activation rows of a tile of the many-token kernels, by the rows that an expert
+// has on average (us a layer of 128 experts of 2048 x 512, 8 of them chosen, bf16;
+// tiles of 16 / 32 / 64 / 128 rows, the best width of each):
+//   bf16 weights    8 rows 175 / 174 / 178 / 183, 25 rows 227 / 196 / 197 / 203, 62
+//                   rows 347 / 264 / 234 / 245, 250 rows of 64 wider experts 816 /
+//                   503 / 343 / 322
+//   4-bit weights   8 rows 84 / 80 / 99 / 160, 62 rows 187 / 142 / 153 / 200, 250
+//                   rows 376 / 251 / 251 / 271
+//   float           12 rows of bf16 weights' place taken by float ones 170 / 170 /
+//                   301; with 4-bit ones 25 rows 127 / 142 / 308
+struct TileRule {
+  int rows;
+};
+TileRule tile_rule(const qm_moe_geom& g) {
+  const double avg = (double)g.rows * g.top_k / g.experts;
+  const bool mx = g.weight_format == QM_W_MX4;
+  if (g.act_dtype != QM_ACT_BF16) return {mx ? 16 : 32};
+  if (mx) return {avg < 256 ? 32 : 64};
+  return {avg < 40 ? 32 : avg < 128 ? 64 : 128};
+}
+// The few-token kernels take the table of slots where the others keep the lists.
 MoeLayout moe_layout(const qm_moe_geom& g) {
   const size_t es = g.act_dtype == QM_ACT_BF16 ? 2 : 4;
   const size_t t = g.rows, ppt = g.top_k + g.shared, pairs = t * ppt;
-  MoeLayout l;
+  const size_t choices = t * g.top_k, hot = choices < (size_t)g.experts ? choices : (size_t)g.experts;
+  MoeLayout l = {};
   size_t at = 0;
   auto take = [&at](size_t n) { const size_t p = at; at += qm_align256(n); return p; };
   l.logits = take(t * (g.experts + 1) * sizeof(double));
-  l.ids = take(t * g.top_k * sizeof(int));
-  l.pair_w = take(pairs * sizeof(float));
-  l.counts = take(g.experts * sizeof(int));
-  l.lists = take((size_t)g.experts * t * sizeof(int));
+  l.meta = take(2 * sizeof(int));
   l.h = take(pairs * g.inter * es);
-  l.part = take(pairs * g.hidden * sizeof(float));
+  if (g.rows <= FEW) {
+    l.counts = take((g.shared + hot) * sizeof(int));          // slot_expert
+    l.lists = take((g.shared + hot) * 16 * sizeof(int));      // slot_pair
+    l.pair_w = take((g.shared + hot) * 16 * sizeof(float));   // slot_w
+  } else {
+    l.bm = tile_rule(g).rows;
+    // every expert's last tile may be part-filled
+    l.max_tiles = (long)(choices / l.bm + hot + g.shared * ((t + l.bm - 1) / l.bm));
+    l.norms = take(qm_route_norms(g.experts));
+    l.ids = take(choices * sizeof(int));
+    l.pair_w = take(pairs * sizeof(float));
+    l.counts = take((g.experts + 1) * sizeof(int));           // and the number of finished workgroups
+    l.lists = take((size_t)g.experts * t * sizeof(int));
+    l.tiles = take(l.max_tiles * sizeof(int2));
+    l.part = take(pairs * g.hidden * es);
+  }
   l.bytes = at;
   return l;
 }
 
 int check_geom(const qm_moe_geom* g, long ldx) {
   if (!g) return qm_fail(QM_ERR_ARG, "qm_moe: null geometry");
-  const int rc = check_route("qm_moe", g->act_dtype, g->rows, g->hidden, g->experts, g->top_k, ldx);
+  const int rc = qm_check_route("qm_moe", g->act_dtype, g->rows, g->hidden, g->experts, g->top_k, ldx);
   if (rc) return rc;
   if (g->inter <= 0 || g->inter % 32 || g->inter > (1 << 20))
     return qm_fail(QM_ERR_ARG, "qm_moe: inter must be a positive multiple of 32 (at most 2^20)");
@@ -418,53 +475,110 @@ int check_geom(const qm_moe_geom* g, long ldx) {
   return QM_OK;
 }
 
-template <typename WF, typename T>
-int launch_ffn(const MoeArgs<T>& A, hipStream_t stream) {
-  constexpr int TN = 1, MT = 2, NW = 8, TD = 2, ND = 4;
-  hipLaunchKernelGGL((moe_up_kernel<WF, T, TN, MT, NW>), dim3((wt_row_tiles(A.inter) + TN - 1) / TN, A.shared + A.experts),
-                     dim3(64 * NW), 0, stream, A);
-  QM_CHECK_LAUNCH();
-  hipLaunchKernelGGL((moe_down_kernel<WF, T, TD, MT, ND>),
-                     dim3((wt_row_tiles(A.hidden) + TD - 1) / TD, A.shared + A.experts), dim3(64 * ND), 0, stream, A);
-  QM_CHECK_LAUNCH();
-  const long n = (long)A.rows * (A.hidden / 4);
+template <typename T>
+int launch_combine(const MoeArgs<T>& A, hipStream_t stream) {
+  const long n = (long)A.rows * (A.hidden / (16 / (int)sizeof(T)));
   hipLaunchKernelGGL(moe_combine_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, A);
   QM_CHECK_LAUNCH();
   return QM_OK;
+}
+
+template <typename WF, typename T, int TN, int TM, int WN, int WM, int S>
+int launch_gemms(const MoeArgs<T>& A, long max_tiles, hipStream_t stream) {
+  using G = SpanGemm<WF, T, TN, TM, WN, WM, S>;
+  constexpr int NT = 64 * WN * WM;
+  const int hn = TN / 2 * WN, dn = TN * WN;
+  const long up = max_tiles * ((wt_row_tiles(A.inter) + hn - 1) / hn), down = max_tiles * ((wt_row_tiles(A.hidden) + dn - 1) / dn);
+  if (up > 0x7fffffffL / NT || down > 0x7fffffffL / NT) return qm_fail(QM_ERR_UNSUPPORTED, "qm_moe: too many tiles for one launch");
+  int rc = qm_allow_lds(reinterpret_cast<const void*>(moe_up_gemm_kernel<WF, T, TN, TM, WN, WM, S>), G::LDS_BYTES);
+  if (!rc) rc = qm_allow_lds(reinterpret_cast<const void*>(moe_down_gemm_kernel<WF, T, TN, TM, WN, WM, S>), G::LDS_BYTES);
+  if (rc) return rc;
+  hipLaunchKernelGGL((moe_up_gemm_kernel<WF, T, TN, TM, WN, WM, S>), dim3((unsigned)up), dim3(NT), G::LDS_BYTES, stream, A);
+  QM_CHECK_LAUNCH();
+  hipLaunchKernelGGL((moe_down_gemm_kernel<WF, T, TN, TM, WN, WM, S>), dim3((unsigned)down), dim3(NT), G::LDS_BYTES, stream, A);
+  QM_CHECK_LAUNCH();
+  return launch_combine(A, stream);
+}
+
+template <typename WF, typename T>
+int launch_ffn(const MoeArgs<T>& A, int bm, long max_tiles, hipStream_t stream) {
+  // (tile_rule)
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (Fmt<WF, T>::SCALED) return launch_gemms<WF, T, 4, 1, 2, 1, 2>(A, max_tiles, stream);
+    else return launch_gemms<WF, T, 2, 2, 4, 1, 2>(A, max_tiles, stream);
+  } else if constexpr (Fmt<WF, T>::SCALED) {
+    return bm == 32 ? launch_gemms<WF, T, 4, 2, 4, 1, 2>(A, max_tiles, stream)
+                    : launch_gemms<WF, T, 2, 4, 4, 1, 2>(A, max_tiles, stream);
+  } else {
+    if (bm == 32) return launch_gemms<WF, T, 2, 2, 4, 1, 3>(A, max_tiles, stream);
+    return bm == 64 ? launch_gemms<WF, T, 2, 4, 4, 1, 3>(A, max_tiles, stream)
+                    : launch_gemms<WF, T, 4, 4, 2, 2, 2>(A, max_tiles, stream);
+  }
+}
+
+template <typename WF, typename T, int PER>
+int launch_few_per(const FewArgs<T>& A, int max_slots, hipStream_t stream) {
+  const dim3 up(wt_row_tiles(A.m.inter), max_slots);
+  if (A.m.rows == 1) {
+    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, PER, true>), up, dim3(64 * FEW_UP_NW), 0, stream, A);
+  } else {
+    hipLaunchKernelGGL((moe_few_plan_kernel<T, PER>), dim3(1), dim3(64 * FEW), 0, stream, A);
+    QM_CHECK_LAUNCH();
+    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, 1, false>), up, dim3(64 * FEW_UP_NW), 0, stream, A);
+  }
+  QM_CHECK_LAUNCH();
+  hipLaunchKernelGGL((moe_few_down_kernel<WF, T>), dim3(wt_row_tiles(A.m.hidden)), dim3(64 * FEW_DOWN_NW), 0, stream, A);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+template <typename WF, typename T>
+int launch_few(const FewArgs<T>& A, hipStream_t stream) {
+  const int choices = A.m.rows * A.m.top_k, slots = A.m.shared + (choices < A.m.experts ? choices : A.m.experts);
+  if (A.m.experts <= 64) return launch_few_per<WF, T, 1>(A, slots, stream);
+  if (A.m.experts <= 128) return launch_few_per<WF, T, 2>(A, slots, stream);
+  if (A.m.experts <= 256) return launch_few_per<WF, T, 4>(A, slots, stream);
+  if (A.m.experts <= 512) return launch_few_per<WF, T, 8>(A, slots, stream);
+  return launch_few_per<WF, T, 16>(A, slots, stream);
 }
 
 template <typename T, typename WPlain>
 int run_moe(const qm_moe_geom& g, const qm_moe_weights& w, const void* x, long ldx, void* out, char* ws,
             hipStream_t stream) {
   const MoeLayout l = moe_layout(g);
-  LogitArgs<T> L = {static_cast<const T*>(x), ldx, static_cast<const T*>(w.router), static_cast<const T*>(w.shared_router),
-                    reinterpret_cast<double*>(ws + l.logits), g.rows, g.hidden, g.experts,
-                    g.experts + (w.shared_router && g.shared ? 1 : 0)};
-  int rc = launch_logits<T>(L, stream);
-  if (rc) return rc;
-  int* ids = reinterpret_cast<int*>(ws + l.ids);
-  float* pair_w = reinterpret_cast<float*>(ws + l.pair_w);
   int* counts = reinterpret_cast<int*>(ws + l.counts);
-  int* lists = reinterpret_cast<int*>(ws + l.lists);
-  const int ppt = g.top_k + g.shared;
-  hipLaunchKernelGGL(moe_topk_kernel, dim3((g.rows + 3) / 4), dim3(256), 0, stream, L.logits, g.rows, L.cols, g.experts,
-                     g.top_k, g.normalize, ids, pair_w, ppt, g.shared);
-  QM_CHECK_LAUNCH();
-  hipLaunchKernelGGL(moe_lists_kernel, dim3(g.experts), dim3(256), 0, stream, ids, g.rows, g.top_k, ppt, counts, lists);
-  QM_CHECK_LAUNCH();
-  MoeArgs<T> A = {};
-  A.x = L.x; A.ldx = ldx; A.rows = g.rows; A.hidden = g.hidden; A.inter = g.inter; A.experts = g.experts;
-  A.shared = g.shared; A.top_k = g.top_k; A.ppt = ppt;
+  const QmLogits<T> L = {static_cast<const T*>(x), ldx, static_cast<const T*>(w.router),
+                         static_cast<const T*>(w.shared_router), reinterpret_cast<double*>(ws + l.logits), g.rows, g.hidden,
+                         g.experts, g.experts + (w.shared_router && g.shared ? 1 : 0), g.rows <= FEW ? nullptr : counts};
   const bool mx = g.weight_format == QM_W_MX4;
   auto mat = [mx](const void* d, const void* s) { return WMat{d, mx ? static_cast<const uint8_t*>(s) : nullptr}; };
+  int* meta = reinterpret_cast<int*>(ws + l.meta);
+  MoeArgs<T> A = {};
+  A.x = L.x; A.ldx = ldx; A.rows = g.rows; A.hidden = g.hidden; A.inter = g.inter; A.experts = g.experts;
+  A.shared = g.shared; A.top_k = g.top_k; A.ppt = g.top_k + g.shared;
   A.gate = mat(w.gate, w.gate_scales); A.up = mat(w.up, w.up_scales); A.down = mat(w.down, w.down_scales);
   A.s_gate = mat(w.shared_gate, w.shared_gate_scales); A.s_up = mat(w.shared_up, w.shared_up_scales);
   A.s_down = mat(w.shared_down, w.shared_down_scales);
-  A.counts = counts; A.lists = lists; A.pair_w = pair_w;
   A.h = reinterpret_cast<T*>(ws + l.h);
-  A.part = reinterpret_cast<float*>(ws + l.part);
   A.out = static_cast<T*>(out);
-  return mx ? launch_ffn<WMx4, T>(A, stream) : launch_ffn<WPlain, T>(A, stream);
+  if (g.rows <= FEW) {
+    const FewArgs<T> P = {A, L.logits, L.cols, g.normalize, meta, counts,
+                          reinterpret_cast<int*>(ws + l.lists), reinterpret_cast<float*>(ws + l.pair_w)};
+    const int rc = qm_route_logits(L, stream);
+    if (rc) return rc;
+    return mx ? launch_few<WMx4, T>(P, stream) : launch_few<WPlain, T>(P, stream);
+  }
+  int* ids = reinterpret_cast<int*>(ws + l.ids);
+  float* pair_w = reinterpret_cast<float*>(ws + l.pair_w);
+  int* lists = reinterpret_cast<int*>(ws + l.lists);
+  int2* tiles = reinterpret_cast<int2*>(ws + l.tiles);
+  const QmRouteLists lists_out = {counts, lists, meta + 1, tiles, A.ppt, g.shared, l.bm};
+  const int rc = qm_route(L, g.top_k, g.normalize, ids, pair_w, A.ppt, g.shared, &lists_out,
+                          reinterpret_cast<float*>(ws + l.norms), stream);
+  if (rc) return rc;
+  A.counts = counts; A.lists = lists; A.pair_w = pair_w; A.n_tiles = meta + 1; A.tiles = tiles;
+  A.part = reinterpret_cast<T*>(ws + l.part);
+  return mx ? launch_ffn<WMx4, T>(A, l.bm, l.max_tiles, stream) : launch_ffn<WPlain, T>(A, l.bm, l.max_tiles, stream);
 }
 
 }  // namespace
@@ -485,38 +599,6 @@ extern "C" int qm_tile_weight(int act_dtype, int mats, int n, int k, const void*
   else
     hipLaunchKernelGGL(tile_weight_kernel<float>, dim3((unsigned)nb), dim3(256), 0, stream, n, k, rt, kt, total,
                        static_cast<const float*>(w), static_cast<char*>(tiles));
-  QM_CHECK_LAUNCH();
-  return QM_OK;
-}
-
-extern "C" size_t qm_moe_route_workspace(int rows, int experts) {
-  if (rows <= 0 || experts <= 0 || experts > RT_MAX_EXPERTS) return 0;
-  return qm_align256((size_t)rows * experts * sizeof(double));
-}
-
-extern "C" int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, int normalize, const void* x,
-                            long ldx, const void* router, int* ids, float* weights, void* workspace,
-                            size_t workspace_bytes, hipStream_t stream) {
-  int rc = check_route("qm_moe_route", act_dtype, rows, hidden, experts, top_k, ldx);
-  if (rc) return rc;
-  if (!x || !router || !ids || !weights || !workspace) return qm_fail(QM_ERR_ARG, "qm_moe_route: null pointer");
-  if (!aligned16(x) || !aligned16(router) || !aligned16(workspace))
-    return qm_fail(QM_ERR_ARG, "qm_moe_route: x, router and workspace must be 16-byte aligned");
-  if (workspace_bytes < qm_moe_route_workspace(rows, experts))
-    return qm_fail(QM_ERR_WORKSPACE, "qm_moe_route: workspace too small");
-  double* logits = static_cast<double*>(workspace);
-  if (act_dtype == QM_ACT_BF16) {
-    LogitArgs<bf16_t> L = {static_cast<const bf16_t*>(x), ldx, static_cast<const bf16_t*>(router), nullptr, logits, rows,
-                           hidden, experts, experts};
-    rc = launch_logits<bf16_t>(L, stream);
-  } else {
-    LogitArgs<float> L = {static_cast<const float*>(x), ldx, static_cast<const float*>(router), nullptr, logits, rows,
-                          hidden, experts, experts};
-    rc = launch_logits<float>(L, stream);
-  }
-  if (rc) return rc;
-  hipLaunchKernelGGL(moe_topk_kernel, dim3((rows + 3) / 4), dim3(256), 0, stream, logits, rows, experts, experts, top_k,
-                     normalize, ids, weights, top_k, 0);
   QM_CHECK_LAUNCH();
   return QM_OK;
 }

@@ -12,7 +12,7 @@
 //
 // Weights are kept in the operand order of wtile.h, 17 bytes for 32 weights.
 #include "qwen4mix_internal.h"
-#include "wtile.h"
+#include "wgemm.h"
 
 namespace {
 
@@ -164,6 +164,24 @@ struct Mx4LinearArgs {
   T* seg_out[QM_GEMV_MAX_SEG];
 };
 
+// outputs n .. n + 3 of row m
+template <typename T>
+__device__ __forceinline__ void store4(const Mx4LinearArgs<T>& A, int m, int n, f32x4_t v) {
+  if (m >= A.m || n >= A.n) return;
+  int s = 0, start = 0;
+  while (s + 1 < A.n_seg && n >= A.seg_end[s]) { start = A.seg_end[s]; ++s; }
+  const int n_s = A.seg_end[s] - start;
+  T* o = A.seg_out[s] + (long)m * n_s + (n - start);
+  if (n + 4 <= A.seg_end[s] && (reinterpret_cast<uintptr_t>(o) & (4 * sizeof(T) - 1)) == 0) {
+    store_act4(o, v);
+    return;
+  }
+  for (int i = 0; i < 4 && n + i < A.n; ++i) {
+    while (s + 1 < A.n_seg && n + i >= A.seg_end[s]) { start = A.seg_end[s]; ++s; }
+    Act<T>::store(A.seg_out[s], (long)m * (A.seg_end[s] - start) + (n + i - start), v[i]);
+  }
+}
+
 template <typename T, int TN, int MT, int NW, int PS>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4LinearArgs<T> A) {
   using F = Fmt<WMx4, T>;
@@ -172,26 +190,21 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4LinearArgs<T> A) {
   const int g4 = lane >> 4, r16 = lane & 15;
   const int t0 = blockIdx.x * TN, m0 = blockIdx.y * 16 * MT;
   f32x4_t acc[TN][MT];
-#pragma unroll
-  for (int t = 0; t < TN; ++t)
-#pragma unroll
-    for (int u = 0; u < MT; ++u) acc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  clear(acc);
   for (int k0 = wid; k0 < A.kt; k0 += NW * PS) {
     typename F::W w[PS][TN];
-    typename F::X x[PS][MT];
+    Acts<F, T> x[PS][MT];
 #pragma unroll
     for (int p = 0; p < PS; ++p) {
       const int ks = min(k0 + p * NW, A.kt - 1);
 #pragma unroll
       for (int t = 0; t < TN; ++t) w[p][t] = F::load_w(A.w, (long)min(t0 + t, A.rt - 1) * A.kt + ks, lane);
-      const int kb = ks * WT_K + g4 * MX_BLOCK;
 #pragma unroll
-      for (int u = 0; u < MT; ++u)
-        x[p][u] = F::load_x(kb < A.k ? A.x + (long)min(m0 + 16 * u + r16, A.m - 1) * A.ldx + kb : nullptr);
+      for (int u = 0; u < MT; ++u) x[p][u].load(A.x + (long)min(m0 + 16 * u + r16, A.m - 1) * A.ldx, ks, A.k, g4);
     }
 #pragma unroll
     for (int p = 0; p < PS; ++p)
-      if (k0 + p * NW < A.kt) F::step(acc, w[p], x[p]);
+      if (k0 + p * NW < A.kt) step_tile<F, T>(acc, w[p], x[p]);
   }
 #pragma unroll
   for (int t = 0; t < TN; ++t)
@@ -202,15 +215,7 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4LinearArgs<T> A) {
     f32x4_t v = s_red[0][r][lane];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += s_red[w][r][lane];
-    const int n = (t0 + r / MT) * 16 + 4 * g4, m = m0 + 16 * (r % MT) + r16;
-    if (m >= A.m) continue;
-    int s = 0, start = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (n + i >= A.n) break;
-      while (s + 1 < A.n_seg && n + i >= A.seg_end[s]) { start = A.seg_end[s]; ++s; }
-      Act<T>::store(A.seg_out[s], (long)m * (A.seg_end[s] - start) + (n + i - start), v[i]);
-    }
+    store4(A, m0 + 16 * (r % MT) + r16, (t0 + r / MT) * 16 + 4 * g4, v);
   }
 }
 
@@ -222,10 +227,75 @@ int launch_rows(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   return QM_OK;
 }
 
+// Many activation rows: a workgroup per 16 TN WN weight rows x 16 TM WM
+// activation rows (wgemm.h), the activation rows' tiles of one range of weights
+// side by side on an XCD.
+template <typename T, int TN, int TM, int WN, int WM, int S>
+__global__ __launch_bounds__(64 * WN * WM, 2) void mx4_gemm_kernel(Mx4LinearArgs<T> A) {
+  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S>;
+  extern __shared__ __attribute__((aligned(16))) char s_buf[];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int mt = (A.m + G::BM - 1) / G::BM;
+  const int item = xcd_run(blockIdx.x, gridDim.x);
+  const int m0 = item % mt * G::BM, t0 = item / mt * WN * TN;
+  auto first = [&](int q) { return (long)min(t0 + q, A.rt - 1) * A.kt; };
+  const typename G::Src src = G::source(
+      wid, lane, [&](int i) { return A.x + (long)min(m0 + i, A.m - 1) * A.ldx; },
+      [&](int q) { return static_cast<const char*>(A.w.data) + first(q) * G::F::TILE; },
+      [&](int q) { return A.w.scales + first(q) * 64; });
+  f32x4_t acc[TN][TM];
+  clear(acc);
+  G::run(acc, s_buf, src, A.k);
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int u = 0; u < TM; ++u)
+      store4(A, m0 + (wid % WM) * 16 * TM + 16 * u + (lane & 15), (t0 + wid / WM * TN + t) * 16 + 4 * (lane >> 4), acc[t][u]);
+}
+
+template <typename T, int TN, int TM, int WN, int WM, int S>
+int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
+  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S>;
+  const long nb = (long)((A.rt + TN * WN - 1) / (TN * WN)) * ((A.m + G::BM - 1) / G::BM);
+  if (nb > 0x7fffffffL / (64 * WN * WM)) return qm_fail(QM_ERR_UNSUPPORTED, "qm_mx4_linear: too many tiles for one launch");
+  const int rc = qm_allow_lds(reinterpret_cast<const void*>(mx4_gemm_kernel<T, TN, TM, WN, WM, S>), G::LDS_BYTES);
+  if (rc) return rc;
+  hipLaunchKernelGGL((mx4_gemm_kernel<T, TN, TM, WN, WM, S>), dim3((unsigned)nb), dim3(64 * WN * WM), G::LDS_BYTES, stream, A);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+// The kernel for m rows (weights from memory, graph replays, us a call):
+//   bf16, up to 16 rows   two row tiles a workgroup where the weight has 256 of them
+//     or more (12352 x 2048: 1 row 5.0, 16 rows 7.3, with one tile 5.4 and 10.2),
+//     else one, two k tiles a wave in flight (2048 x 4096: 1 row 3.9, 14 rows 6.0,
+//     with two tiles 4.5 and 6.4)
+//   bf16, more rows   the largest of the tiles of wgemm.h that makes 256 workgroups
+//     (160 for the smallest). 12352 x 2048, 256 x 64 / 256 x 32 / 128 x 32 / 128 x 16
+//     tiles: 64 rows 26 / 16.6 / 11.7 / 10.6, 128 rows 26 / 16.8 / 13.8 / 18.1, 256
+//     rows 26 / 22.0 / 25.6 / 26.8, 512 rows 34.6 / 40.2 / 39.8 / 50. Fewer
+//     workgroups than that: the few-row kernel with k split over 16 waves (2048 x
+//     4096: 64 rows 7.1 against 14.4, 128 rows 12.1 against 14.5)
+//   float   the same with the smallest tile alone (its activations are cut into
+//     parts by every workgroup: 12352 x 2048, 64 rows 31 against 37 with 32 rows a
+//     tile, 256 rows 88 against 99)
 template <typename T>
 int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
-  if (A.m <= 16) return launch_rows<T, 1, 1, 8, 2>(A, stream);
-  return launch_rows<T, 2, 2, 8, 1>(A, stream);
+  auto groups = [&A](int bn, int bm) { return (long)((A.rt * 16 + bn - 1) / bn) * ((A.m + bm - 1) / bm); };
+  if (A.m <= 16) {
+    if (A.rt >= 256) return launch_rows<T, 2, 1, 8, 1>(A, stream);
+    return launch_rows<T, 1, 1, 8, 2>(A, stream);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (groups(256, 64) >= 256) return launch_gemm<T, 4, 4, 4, 1, 2>(A, stream);
+    if (groups(256, 32) >= 256) return launch_gemm<T, 4, 2, 4, 1, 2>(A, stream);
+    if (groups(128, 32) >= 256) return launch_gemm<T, 2, 2, 4, 1, 3>(A, stream);
+    if (groups(128, 16) >= 160) return launch_gemm<T, 2, 1, 4, 1, 4>(A, stream);
+    return launch_rows<T, 2, 1, 16, 1>(A, stream);
+  } else {
+    if (groups(128, 16) >= 256) return launch_gemm<T, 2, 1, 4, 1, 3>(A, stream);
+    return launch_rows<T, 2, 1, 8, 1>(A, stream);
+  }
 }
 
 bool mx_sizes_ok(int mats, int n, int k) {

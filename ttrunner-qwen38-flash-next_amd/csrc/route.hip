@@ -1,0 +1,512 @@
+// Routing of token rows to experts, gfx950 (reference/model.py:387-417):
+//
+//   l[t][e] = sum_k x[t][k] R[e][k]            ids[t] = the top_k largest, ties to the lower index
+//   w[t][j] = softmax(l[t])[ids[t][j]]         (over the chosen ones alone when normalize)
+//
+// The choice is that of the logits summed in double: which experts a token takes
+// then depends on its values alone, not on the number of rows beside it or the
+// order of a float sum, so a verify step routes as the single steps do.
+//
+// Few rows form those sums outright, a wave per router row. Many rows take the
+// matrix cores: products of 128 k are summed in float, the sums of 128 in double,
+// so a logit is off by at most
+//     B = (129 2^-23) |x| |R[e]| + hidden 2^-126      (|.| the 2-norms; the last
+// for products below float's range), and only where two of a token's leading
+// logits come closer than 2 B can the order be another. Those logits alone are
+// summed again in double (about one token in ten of normal rows has such a pair).
+#include "moe_internal.h"
+#include "moe_topk.h"
+#include "wtile.h"
+
+namespace {
+
+constexpr double ROUTE_FEW = 1e8;
+constexpr int RT_TB = 4;                 // token rows of one wave of the few-row logits
+
+// 16 bytes as floats
+__device__ __forceinline__ void unit_get(const uint4& c, float (&v)[8], const bf16_t*) {
+  const unsigned d[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(d[i] << 16);
+    v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unit_get(const uint4& c, float (&v)[4], const float*) {
+  v[0] = __uint_as_float(c.x); v[1] = __uint_as_float(c.y); v[2] = __uint_as_float(c.z); v[3] = __uint_as_float(c.w);
+}
+
+// s + w x in double: a product of bf16 is exact in float
+__device__ __forceinline__ double exact_fma(float w, float x, double s, const bf16_t*) { return s + (double)(w * x); }
+__device__ __forceinline__ double exact_fma(float w, float x, double s, const float*) { return fma((double)w, (double)x, s); }
+
+template <int LANES> __device__ __forceinline__ double lanes_sum_f64(double v) {
+#pragma unroll
+  for (int m = LANES / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* router_row(const QmLogits<T>& A, int r) {
+  return r < A.experts ? A.router + (long)r * A.hidden : A.shared_router;
+}
+
+// The square of a row's norm from partial sums of squares and largest magnitudes
+// over groups of lanes: zero only of a row of zeros, infinite where a NaN or an
+// infinity is in it.
+__device__ __forceinline__ float guard_norm(float sq, float big) {
+  if (sq != sq) return INFINITY;
+  return big != 0.f ? fmaxf(sq, 0x1p-126f) : sq;
+}
+__device__ __forceinline__ float oct_norm(float sq, float big) {
+#pragma unroll
+  for (int m = 1; m <= 4; m <<= 1) {
+    sq += __shfl_xor(sq, m, 64);
+    big = fmaxf(big, __shfl_xor(big, m, 64));
+  }
+  return guard_norm(sq, big);
+}
+
+// the experts' counts of pairs, for the choice that follows
+template <typename T> __device__ __forceinline__ void clear_counts(const QmLogits<T>& A) {
+  if (A.counts && blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i <= A.experts; i += blockDim.x) A.counts[i] = 0;
+}
+
+// logits[t][r] of the router's rows and, when there is one, the shared experts' row
+template <typename T>
+__global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
+  constexpr int VE = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  clear_counts(A);
+  if (r >= A.cols) return;
+  const int t0 = blockIdx.y * RT_TB;
+  const T* w = router_row(A, r);
+  double acc[RT_TB];
+#pragma unroll
+  for (int i = 0; i < RT_TB; ++i) acc[i] = 0.0;
+  for (int u = lane; u < A.hidden / VE; u += 64) {
+    float wv[VE];
+    unit_get(*reinterpret_cast<const uint4*>(w + (long)u * VE), wv, w);
+#pragma unroll
+    for (int i = 0; i < RT_TB; ++i) {
+      if (t0 + i >= A.rows) break;
+      float xv[VE];
+      unit_get(*reinterpret_cast<const uint4*>(A.x + (long)(t0 + i) * A.ldx + (long)u * VE), xv, w);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[i] = exact_fma(wv[e], xv[e], acc[i], w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RT_TB; ++i) {
+    const double s = lanes_sum_f64<64>(acc[i]);
+    if (lane == 0 && t0 + i < A.rows) A.logits[(long)(t0 + i) * A.cols + r] = s;
+  }
+}
+
+// The same by matrix cores: a workgroup per 64 router rows x 64 tokens, both kinds
+// of rows in LDS (128 k of each at a time, units exchanged as in wgemm.h), a wave
+// per 32 x 32. norms: |R[r]|^2, by the workgroups of the first tokens.
+constexpr int LG_ROWS = 128;
+template <typename T> constexpr int LG_S = sizeof(T) == 2 ? 4 : 2;
+
+template <typename T>
+__global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, float* norms) {
+  constexpr int ROW_B = WT_K * sizeof(T), UNITS = ROW_B / 16, VE = 16 / sizeof(T), RPL = 1024 / ROW_B;
+  constexpr int LOADS = LG_ROWS / RPL / 8, BUF = LG_ROWS * ROW_B, S = LG_S<T>;
+  extern __shared__ __attribute__((aligned(16))) char s_buf[];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g4 = lane >> 4, r16 = lane & 15;
+  const int e0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
+  const T* src[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int row = (wid * LOADS + i) * RPL + lane / UNITS;
+    src[i] = row < 64 ? router_row(A, min(e0 + row, A.cols - 1)) : A.x + (long)min(t0 + row - 64, A.rows - 1) * A.ldx;
+  }
+  auto fetch = [&](int j) {
+    char* buf = s_buf + j % S * BUF;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = (wid * LOADS + i) * RPL + lane / UNITS;
+      const int k = j * WT_K + ((lane % UNITS) ^ (row & 15)) * VE;
+      lds_load16(k < A.hidden ? static_cast<const void*>(src[i] + k) : g_zero_unit, buf + (wid * LOADS + i) * 1024);
+    }
+  };
+  const int spans = wt_k_tiles(A.hidden);
+  clear_counts(A);
+#pragma unroll
+  for (int j = 0; j < S - 1; ++j)
+    if (j < spans) fetch(j);
+  double acc[2][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[u][i] = 0.0;
+  // thread: an eighth of router row tid / 8
+  const int n_row = threadIdx.x >> 3;
+  const bool norm = blockIdx.y == 0;
+  float sq = 0.f, big = 0.f;
+  for (int j = 0; j < spans; ++j) {
+    if (j + S - 2 < spans) wave_loads_barrier<(S - 2) * LOADS>();
+    else wave_loads_barrier<0>();
+    if (j + S - 1 < spans) fetch(j + S - 1);
+    const char* buf = s_buf + j % S * BUF;
+    Piece<T> a[4], b[4][2];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      a[s] = lds_piece<T>(buf + ((wid >> 1) * 16 + r16) * ROW_B, 4 * s + g4, r16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        b[s][h] = lds_piece<T>(buf + (64 + (wid & 1) * 32 + 16 * h + r16) * ROW_B, 4 * s + g4, r16);
+    }
+    __builtin_amdgcn_sched_barrier(0);                       // all reads in flight before the first product
+    f32x4_t part[1][2];
+    clear(part);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) part[0][u] = mma_piece(a[s], b[s][u], part[0][u]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
+    if (norm) {
+      for (int u = 0; u < UNITS / 8; ++u) {                  // each row from another unit on: other banks
+        const int at = (threadIdx.x & 7) * (UNITS / 8) + (u + n_row) % (UNITS / 8);
+        float v[VE];
+        unit_get(*reinterpret_cast<const uint4*>(buf + n_row * ROW_B + at * 16), v, static_cast<const T*>(nullptr));
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          sq = fmaf(v[e], v[e], sq);
+          big = fmaxf(big, fabsf(v[e]));
+        }
+      }
+    }
+  }
+  if (norm) {
+    sq = oct_norm(sq, big);
+    if ((threadIdx.x & 7) == 0 && e0 + n_row < A.cols) norms[e0 + n_row] = sq;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = t0 + (wid & 1) * 32 + 16 * u + r16;
+    if (t >= A.rows) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = e0 + (wid >> 1) * 16 + 4 * g4 + i;
+      if (r < A.cols) A.logits[(long)t * A.cols + r] = acc[u][i];
+    }
+  }
+}
+
+struct TopArgs {
+  int top_k, normalize, ld_w, shared;
+  int* ids;            // [rows][top_k]
+  float* weights;      // [rows][ld_w]: the choices, then the shared experts
+  QmRouteLists lists;  // counts null: none wanted
+  const float* norms;  // null: the logits are sums in double already
+};
+
+// The logit of expert e in double, by 32 lanes
+template <typename T>
+__device__ __forceinline__ double exact_logit(const QmLogits<T>& A, int t, int e, int l32) {
+  constexpr int VE = 16 / sizeof(T);
+  const T* w = A.router + (long)e * A.hidden;
+  const T* x = A.x + (long)t * A.ldx;
+  constexpr int B = 8;                     // loads in flight: the sum is a chain of latencies otherwise
+  const int units = A.hidden / VE;
+  double s = 0.0;
+  for (int u0 = l32; u0 < units; u0 += 32 * B) {
+    uint4 wu[B], xu[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const long at = (long)min(u0 + 32 * b, units - 1) * VE;
+      wu[b] = *reinterpret_cast<const uint4*>(w + at);
+      xu[b] = *reinterpret_cast<const uint4*>(x + at);
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (u0 + 32 * b >= units) break;
+      float wv[VE], xv[VE];
+      unit_get(wu[b], wv, w);
+      unit_get(xu[b], xv, w);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s = exact_fma(wv[i], xv[i], s, w);
+    }
+  }
+  return lanes_sum_f64<32>(s);
+}
+
+// The workgroup that finishes last makes the table of row tiles from the counts,
+// the shared experts first.
+__device__ __forceinline__ void finish_lists(int rows, int experts, const QmRouteLists& L) {
+  __shared__ int s_wave[4];
+  __shared__ bool s_last;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  wait_all_memory();                                         // this wave's counts are in
+  __syncthreads();
+  if (threadIdx.x == 0)
+    s_last = __hip_atomic_fetch_add(L.counts + experts, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  int start = 0;
+  const int all = L.shared + experts;
+  for (int y0 = 0; y0 < all; y0 += 256) {
+    const int y = y0 + threadIdx.x;
+    int count = 0;
+    if (y < all) count = y < L.shared ? rows : (int)ld_flag(reinterpret_cast<const unsigned*>(L.counts + y - L.shared));
+    const int mine = (count + L.bm - 1) / L.bm;
+    int before = mine;                                       // inclusive scan over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(before, d, 64);
+      if (lane >= d) before += o;
+    }
+    __syncthreads();
+    if (lane == 63) s_wave[wid] = before;
+    __syncthreads();
+    int place = start + before - mine;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int c = s_wave[w];
+      if (w < wid) place += c;
+      start += c;
+    }
+    for (int i = 0; i < mine; ++i) L.tiles[place + i] = make_int2(y, i * L.bm);
+  }
+  if (threadIdx.x == 0) *L.n_tiles = start;
+}
+
+// A token's choice, by one wave
+template <typename T, int PER>
+__device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P, int t, int lane) {
+  double* l = A.logits + (long)t * A.cols;
+  WaveTop<PER> top;
+  float sq = 0.f, big = 0.f;               // of the token's row
+  if (P.norms) {
+    constexpr int VE = 16 / sizeof(T);
+    for (int u = lane; u < A.hidden / VE; u += 64) {
+      float v[VE];
+      unit_get(*reinterpret_cast<const uint4*>(A.x + (long)t * A.ldx + (long)u * VE), v, A.x);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        sq = fmaf(v[i], v[i], sq);
+        big = fmaxf(big, fabsf(v[i]));
+      }
+    }
+  }
+  top.load(l, A.experts, lane);
+  // 2 B: logits further apart are in the right order
+  double close = -1.0;
+  bool all = false;                        // every logit has to be summed again
+  if (P.norms) {
+    float wn = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane + 64 * i;
+      if (e >= A.experts) continue;
+      const float v = P.norms[e];
+      wn = fmaxf(wn, v);
+      bad |= !(v < INFINITY) || !(fabs(l[e]) < (double)INFINITY);
+    }
+    const float xn = guard_norm(wave_sum(sq), wave_max(big));
+    wn = wave_max(wn);
+    // squares below float's range hide a norm
+    all = __builtin_amdgcn_ballot_w64(bad) != 0ull || !(xn < INFINITY) || (xn != 0.f && (xn < 0x1p-80f || wn < 0x1p-80f));
+    // (a row of zeros has logits of zero; the norms' own rounding is far below 2^-10)
+    if (all) close = 0.0;
+    else if (xn != 0.f) close = 2.0 * (129.0 * 0x1p-23 * (1.0 + 0x1p-10) * sqrt((double)xn * (double)wn) + A.hidden * 0x1p-126);
+  }
+  int n = 0, id = 0x7fffffff;
+  long long key = KEY_GONE;                // lane j: the j-th largest
+  if (!all) {
+    double bar = 0.0;                      // the top_k-th logit - 2 B
+    const int most = close < 0.0 ? P.top_k : A.experts;
+    for (; n < most; ++n) {
+      long long best;
+      const int at = top.take(lane, best);
+      const double v = key_logit(best);
+      if (n == P.top_k - 1) bar = v - close;
+      if (n >= P.top_k && v < bar) break;
+      if (n == 64) { all = true; break; }  // more candidates than lanes
+      if (lane == n) { key = best; id = at; }
+    }
+  }
+  if (close >= 0.0) {
+    if (!all) {
+      // neighbours closer than 2 B: both in double
+      const double v = key_logit(key), above = __shfl_up(v, 1, 64), below = __shfl_down(v, 1, 64);
+      const bool again = lane < n && ((lane > 0 && above - v <= close) || (lane + 1 < n && v - below <= close));
+      const unsigned long long close_ones = __builtin_amdgcn_ballot_w64(again);
+      unsigned long long m = close_ones;
+      while (m) {
+        // two at a time; the other half repeats the first where there is one
+        const int first = __ffsll(m) - 1;
+        m &= m - 1;
+        const int second = m ? __ffsll(m) - 1 : first;
+        m &= m - 1;
+        const int e = lane < 32 ? __builtin_amdgcn_readlane(id, first) : __builtin_amdgcn_readlane(id, second);
+        const double s = exact_logit(A, t, e, lane & 31);
+        const long long k = logit_key(s);
+        const long long k0 = lane_key(k, 0), k1 = lane_key(k, 32);
+        if (lane == first) key = k0;
+        if (lane == second) key = k1;
+      }
+      // their order again
+      int rank = 0;
+      for (int i = 0; close_ones && i < n; ++i) {
+        const long long ok = lane_key(key, i);
+        const int oi = __builtin_amdgcn_readlane(id, i);
+        rank += ok > key || (ok == key && oi < id);
+      }
+      long long sorted_key = key;
+      int sorted_id = id;
+      for (int i = 0; close_ones && i < n; ++i) {
+        const int at = __builtin_amdgcn_readlane(rank, i);
+        const long long ok = lane_key(key, i);
+        const int oi = __builtin_amdgcn_readlane(id, i);
+        if (lane == at) { sorted_key = ok; sorted_id = oi; }
+      }
+      key = sorted_key;
+      id = sorted_id;
+    } else {
+      for (int e0 = 0; e0 < A.experts; e0 += 2) {
+        const int e = min(e0 + (lane >> 5), A.experts - 1);
+        const double s = exact_logit(A, t, e, lane & 31);
+        if ((lane & 31) == 0 && e0 + (lane >> 5) < A.experts) l[e] = s;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      wait_all_memory();
+      top.load(l, A.experts, lane);
+      for (n = 0; n < P.top_k; ++n) {
+        long long best;
+        const int at = top.take(lane, best);
+        if (lane == n) { key = best; id = at; }
+      }
+    }
+  }
+  const double v0 = key_logit(lane_key(key, 0));
+  const float mine = lane < P.top_k ? expf((float)(key_logit(key) - v0)) : 0.f;
+  float sum = 0.f;
+  if (P.normalize) {
+    sum = wave_sum(mine);
+  } else {
+    for (int e = lane; e < A.experts; e += 64) sum += expf((float)(l[e] - v0));
+    sum = wave_sum(sum);
+  }
+  if (lane < P.top_k) {
+    P.ids[(long)t * P.top_k + lane] = id;
+    P.weights[(long)t * P.ld_w + lane] = mine / sum;
+    if (P.lists.counts) {
+      // the order of an expert's pairs is that of arrival; their products do not
+      // depend on it
+      const int at = __hip_atomic_fetch_add(P.lists.counts + id, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      P.lists.lists[(long)id * A.rows + at] = t * P.lists.ppt + lane;
+    }
+  }
+  if (lane < P.shared)
+    P.weights[(long)t * P.ld_w + P.top_k + lane] = A.cols > A.experts ? sigmoid_f((float)l[A.experts]) : 1.f;
+}
+
+// One wave per token
+template <typename T, int PER>
+__global__ __launch_bounds__(256) void moe_topk_kernel(QmLogits<T> A, TopArgs P) {
+  const int lane = threadIdx.x & 63;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t < A.rows) topk_row<T, PER>(A, P, t, lane);
+  if (P.lists.counts) finish_lists(A.rows, A.experts, P.lists);
+}
+
+template <typename T, int PER>
+int launch_topk(const QmLogits<T>& A, const TopArgs& P, hipStream_t stream) {
+  hipLaunchKernelGGL((moe_topk_kernel<T, PER>), dim3((A.rows + 3) / 4), dim3(256), 0, stream, A, P);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+size_t qm_route_norms(int experts) { return ((size_t)experts + 1) * sizeof(float); }
+
+template <typename T>
+int qm_route_logits(const QmLogits<T>& A, hipStream_t stream) {
+  hipLaunchKernelGGL(moe_logits_kernel<T>, dim3((A.cols + 3) / 4, (A.rows + RT_TB - 1) / RT_TB), dim3(256), 0, stream, A);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
+}
+
+template <typename T>
+int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* weights, int ld_w, int shared,
+             const QmRouteLists* lists, float* norms, hipStream_t stream) {
+  TopArgs P = {top_k, normalize, ld_w, shared, ids, weights, lists ? *lists : QmRouteLists{}, nullptr};
+  int rc;
+  if ((double)A.rows * A.cols * A.hidden <= ROUTE_FEW) {
+    rc = qm_route_logits(A, stream);
+  } else {
+    P.norms = norms;
+    const size_t lds = (size_t)LG_S<T> * LG_ROWS * WT_K * sizeof(T);
+    rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64, (A.rows + 63) / 64), dim3(512), lds, stream, A, norms);
+    QM_CHECK_LAUNCH();
+  }
+  if (rc) return rc;
+  if (A.experts <= 64) return launch_topk<T, 1>(A, P, stream);
+  if (A.experts <= 128) return launch_topk<T, 2>(A, P, stream);
+  if (A.experts <= 256) return launch_topk<T, 4>(A, P, stream);
+  if (A.experts <= 512) return launch_topk<T, 8>(A, P, stream);
+  return launch_topk<T, 16>(A, P, stream);
+}
+
+template int qm_route_logits<bf16_t>(const QmLogits<bf16_t>&, hipStream_t);
+template int qm_route_logits<float>(const QmLogits<float>&, hipStream_t);
+template int qm_route<bf16_t>(const QmLogits<bf16_t>&, int, int, int*, float*, int, int, const QmRouteLists*, float*, hipStream_t);
+template int qm_route<float>(const QmLogits<float>&, int, int, int*, float*, int, int, const QmRouteLists*, float*, hipStream_t);
+
+int qm_check_route(const char* what, int act_dtype, int rows, int hidden, int experts, int top_k, long ldx) {
+  char msg[160];
+  const int unit = act_dtype == QM_ACT_BF16 ? 8 : 4;
+  const char* bad = nullptr;
+  int code = QM_ERR_ARG;
+  if (act_dtype != QM_ACT_BF16 && act_dtype != QM_ACT_F32) { bad = "act_dtype must be QM_ACT_F32 or QM_ACT_BF16"; code = QM_ERR_DTYPE; }
+  else if (rows <= 0 || rows > 262140) bad = "rows must be 1..262140";
+  else if (hidden <= 0 || hidden % 32 || hidden > (1 << 20)) bad = "hidden must be a positive multiple of 32 (at most 2^20)";
+  else if (experts <= 0 || experts > RT_MAX_EXPERTS) { bad = "experts must be 1..1024"; code = QM_ERR_UNSUPPORTED; }
+  else if (top_k <= 0 || top_k > RT_MAX_TOPK || top_k > experts) bad = "top_k must be 1..32 and at most experts";
+  else if (ldx < hidden || ldx % unit) bad = "ldx must be at least hidden and whole 16-byte units";
+  if (!bad) return QM_OK;
+  snprintf(msg, sizeof(msg), "%s: %s", what, bad);
+  return qm_fail(code, msg);
+}
+
+extern "C" size_t qm_moe_route_workspace(int rows, int experts) {
+  if (rows <= 0 || experts <= 0 || experts > RT_MAX_EXPERTS) return 0;
+  return qm_align256((size_t)rows * experts * sizeof(double)) + qm_align256(qm_route_norms(experts));
+}
+
+extern "C" int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, int normalize, const void* x,
+                            long ldx, const void* router, int* ids, float* weights, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream) {
+  const int rc = qm_check_route("qm_moe_route", act_dtype, rows, hidden, experts, top_k, ldx);
+  if (rc) return rc;
+  if (!x || !router || !ids || !weights || !workspace) return qm_fail(QM_ERR_ARG, "qm_moe_route: null pointer");
+  if (!aligned16(x) || !aligned16(router) || !aligned16(workspace))
+    return qm_fail(QM_ERR_ARG, "qm_moe_route: x, router and workspace must be 16-byte aligned");
+  if (workspace_bytes < qm_moe_route_workspace(rows, experts))
+    return qm_fail(QM_ERR_WORKSPACE, "qm_moe_route: workspace too small");
+  double* logits = static_cast<double*>(workspace);
+  float* norms = reinterpret_cast<float*>(static_cast<char*>(workspace) + qm_align256((size_t)rows * experts * sizeof(double)));
+  if (act_dtype == QM_ACT_BF16) {
+    const QmLogits<bf16_t> L = {static_cast<const bf16_t*>(x), ldx, static_cast<const bf16_t*>(router), nullptr, logits, rows,
+                                hidden, experts, experts, nullptr};
+    return qm_route(L, top_k, normalize, ids, weights, top_k, 0, nullptr, norms, stream);
+  }
+  const QmLogits<float> L = {static_cast<const float*>(x), ldx, static_cast<const float*>(router), nullptr, logits, rows,
+                             hidden, experts, experts, nullptr};
+  return qm_route(L, top_k, normalize, ids, weights, top_k, 0, nullptr, norms, stream);
+}

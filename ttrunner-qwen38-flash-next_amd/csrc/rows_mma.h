@@ -79,20 +79,3 @@ __device__ __forceinline__ void to_frags(uint4* lds, const u32x4_t (&rows)[16], 
 #pragma unroll
   for (int i = 0; i < 16; ++i) f[i] = *reinterpret_cast<const u32x4_t*>(lds + r16 * ROW_US + 4 * i + g4);
 }
-
-// 4 consecutive activations as float, and back
-__device__ __forceinline__ void load_act4(const bf16_t* p, float (&v)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-  v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-}
-__device__ __forceinline__ void load_act4(const float* p, float (&v)[4]) {
-  const float4 u = *reinterpret_cast<const float4*>(p);
-  v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-}
-__device__ __forceinline__ void store_act4(bf16_t* p, const float (&v)[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-}
-__device__ __forceinline__ void store_act4(float* p, const float (&v)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}

@@ -66,6 +66,13 @@ int qm_resident_workgroups(const void* kernel, int block_threads, size_t dyn_lds
   return QM_OK;
 }
 
+int qm_allow_lds(const void* kernel, size_t dyn_lds) {
+  if (dyn_lds <= 64 * 1024) return QM_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn_lds);
+  if (e != hipSuccess) return qm_fail(QM_ERR_LAUNCH, hipGetErrorString(e));
+  return QM_OK;
+}
+
 int qm_zero_words(void* p, long n_words, hipStream_t stream) {
   if (n_words <= 0) return QM_OK;
   const int nt = 256;

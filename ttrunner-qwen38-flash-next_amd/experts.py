@@ -17,14 +17,14 @@ import ctypes
 import torch
 
 from . import native
-from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, on_device
+from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, on_device, stream_of
 
 MAX_EXPERTS, MAX_TOP_K, MAX_SHARED = 1024, 32, 32
 
 
 def _check_router(x: torch.Tensor, router: torch.Tensor, top_k: int) -> None:
     experts, hidden = router.shape
-    if x.dim() < 1 or x.shape[-1] != hidden:
+    if x.dim() == 0 or x.shape[-1] != hidden:
         raise ValueError(f"x must be [..., {hidden}], got {tuple(x.shape)}")
     if x.dtype != router.dtype or x.device != router.device:
         raise ValueError(f"x is {x.dtype} on {x.device}, the router {router.dtype} on {router.device}")
@@ -51,22 +51,24 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool
     over all experts, or over the chosen ones when ``normalize``. The logits are
     summed in float64, so that a token's experts do not depend on the rows beside
     it."""
-    check_input(x, "x")
+    act = check_input(x, "x")
     _check_router_shape(router)
     _check_router(x, router, top_k)
     experts, hidden = router.shape
-    ids = torch.empty(*x.shape[:-1], top_k, dtype=torch.int32, device=x.device)
-    weights = torch.empty(*x.shape[:-1], top_k, dtype=torch.float32, device=x.device)
-    m = x.numel() // hidden
+    lead, device = x.shape[:-1], x.device
+    ids = torch.empty(lead + (top_k,), dtype=torch.int32, device=device)
+    weights = torch.empty(lead + (top_k,), dtype=torch.float32, device=device)
+    m = lead.numel()
     if m:
+        lib = native.load()
         xr, ldx = activation_rows(x)
         rc = dense(router)
-        nbytes = native.load().qm_moe_route_workspace(m, experts)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        with on_device(x.device):
-            native.call("qm_moe_route", native.act_code(x.dtype), m, hidden, experts, top_k, int(bool(normalize)),
-                        native.ptr(xr), ldx, native.ptr(rc), native.ptr(ids), native.ptr(weights), native.ptr(ws),
-                        nbytes, native.stream_handle(x.device))
+        nbytes = lib.qm_moe_route_workspace(m, experts)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        with on_device(device):
+            native.check("qm_moe_route", lib.qm_moe_route(
+                act, m, hidden, experts, top_k, 1 if normalize else 0, xr.data_ptr(), ldx, rc.data_ptr(), ids.data_ptr(),
+                weights.data_ptr(), ws.data_ptr(), nbytes, stream_of(device)))
     return ids, weights
 
 
@@ -82,7 +84,7 @@ class _Tiles:
         self.scales = None
         with on_device(w.device):
             native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), native.ptr(self.codes),
-                        native.stream_handle(w.device))
+                        stream_of(w.device))
 
 
 class MoeWeights:
@@ -129,6 +131,7 @@ class MoeWeights:
         s = [None if t is None or t.scales is None else t.scales.data_ptr() for t in mats]
         self._ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
                                           native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
+        self._ptrs_ref = ctypes.byref(self._ptrs)
 
     def _take(self, mats: int, parts, what: str) -> list:
         out = []
@@ -158,6 +161,7 @@ class MoeWeights:
         return self.router.device
 
     def geom(self, rows: int) -> native.MoeGeom:
+        """The geometry of a call of ``rows`` tokens (include/qwen4mix.h)."""
         return native.MoeGeom(rows, self.hidden, self.inter, self.experts, self.shared, self.top_k,
                               int(self.normalize), native.act_code(self.dtype),
                               native.QM_W_MX4 if self.is_mx4 else native.QM_W_ACT)
@@ -168,14 +172,16 @@ def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
     the weighted sum of each token's experts plus its shared experts."""
     check_input(x, "x")
     _check_router(x, weights.router, weights.top_k)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    m = x.numel() // weights.hidden
+    device = x.device
+    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    m = x.shape[:-1].numel()
     if m:
+        lib = native.load()
         xr, ldx = activation_rows(x)
-        g = weights.geom(m)
-        nbytes = native.load().qm_moe_workspace(ctypes.byref(g))
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-        with on_device(x.device):
-            native.call("qm_moe", ctypes.byref(g), ctypes.byref(weights._ptrs), native.ptr(xr), ldx, native.ptr(out),
-                        native.ptr(ws), nbytes, native.stream_handle(x.device))
+        g = ctypes.byref(weights.geom(m))
+        nbytes = lib.qm_moe_workspace(g)
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        with on_device(device):
+            native.check("qm_moe", lib.qm_moe(g, weights._ptrs_ref, xr.data_ptr(), ldx, out.data_ptr(), ws.data_ptr(),
+                                              nbytes, stream_of(device)))
     return out

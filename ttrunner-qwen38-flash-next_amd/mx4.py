@@ -27,20 +27,30 @@ BLOCK = 32
 TILE_ROWS, TILE_K = 16, 128
 
 
+_HERE = contextlib.nullcontext()
+_ACT = {torch.float32: native.QM_ACT_F32, torch.bfloat16: native.QM_ACT_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def on_device(device):
     """A context in which ``device`` is the current one (launches go there)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def check_input(t: torch.Tensor, what: str) -> None:
-    """float32 or bfloat16 on the GPU, and nothing that would lose a gradient."""
+def stream_of(device) -> int:
+    """The handle of the device's current stream."""
+    return _raw_stream(device.index)
+
+
+def check_input(t: torch.Tensor, what: str) -> int:
+    """The type code of a float32 or bfloat16 tensor on the GPU that loses no
+    gradient here."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a tensor on the GPU")
-    native.act_code(t.dtype)
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} requires a gradient, and this operator has none (use torch.no_grad())")
+    code = _ACT.get(t.dtype)
+    return native.act_code(t.dtype) if code is None else code
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:
@@ -53,6 +63,8 @@ def activation_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """x [..., K] as rows [M, K] and the elements from one to the next: a view
     where the kernels can read it (whole 16-byte units), else a copy."""
     k = x.shape[-1]
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, k
     rows = x.reshape(-1, k)
     if rows.stride(1) == 1 and rows.data_ptr() % 16 == 0:
         if rows.shape[0] == 1:
@@ -113,7 +125,7 @@ class Mx4Weight:
         pc, ps = dense(codes), scales.contiguous()
         with on_device(codes.device):
             native.call("qm_mx4_layout", 1, w.mats, shape[-2], shape[-1], native.ptr(w.codes), native.ptr(w.scales),
-                        native.ptr(pc), native.ptr(ps), native.stream_handle(codes.device))
+                        native.ptr(pc), native.ptr(ps), stream_of(codes.device))
         return w
 
     def plain(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -123,7 +135,7 @@ class Mx4Weight:
         scales = torch.empty(*lead, n, k // BLOCK, dtype=torch.uint8, device=self.device)
         with on_device(self.device):
             native.call("qm_mx4_layout", 0, self.mats, n, k, native.ptr(self.codes), native.ptr(self.scales),
-                        native.ptr(codes), native.ptr(scales), native.stream_handle(self.device))
+                        native.ptr(codes), native.ptr(scales), stream_of(self.device))
         return codes, scales
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -133,7 +145,7 @@ class Mx4Weight:
         with on_device(self.device):
             native.call("qm_mx4_dequantize", native.act_code(dtype), self.mats, self.shape[-2], self.shape[-1],
                         native.ptr(self.codes), native.ptr(self.scales), native.ptr(out),
-                        native.stream_handle(self.device))
+                        stream_of(self.device))
         return out
 
 
@@ -147,7 +159,7 @@ def mx4_quantize(w: torch.Tensor) -> Mx4Weight:
     wc = dense(w)
     with on_device(w.device):
         native.call("qm_mx4_quantize", native.act_code(w.dtype), out.mats, w.shape[-2], w.shape[-1], native.ptr(wc),
-                    native.ptr(out.codes), native.ptr(out.scales), native.stream_handle(w.device))
+                    native.ptr(out.codes), native.ptr(out.scales), stream_of(w.device))
     return out
 
 
@@ -157,25 +169,30 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Weight, sections=None):
     ``sections``, a list of row counts that add up to n, splits the rows over
     outputs of their own (the projections of one input kept as one weight): a
     list of [..., rows] tensors is returned."""
-    check_input(x, "x")
+    act = check_input(x, "x")
     if not isinstance(weight, Mx4Weight) or len(weight.shape) != 2:
         raise ValueError("mx4_linear takes a 4-bit weight of one matrix [n, k]")
     n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
-    if x.device != weight.device:
-        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    rows = [n] if sections is None else [int(r) for r in sections]
-    if min(rows, default=0) <= 0 or sum(rows) != n or len(rows) > 8:
-        raise ValueError(f"sections must be 1 to 8 positive row counts that add up to {n}, got {rows}")
-    outs = [torch.empty(*x.shape[:-1], r, dtype=x.dtype, device=x.device) for r in rows]
-    m = x.numel() // k
+    lead = x.shape
+    if not lead or lead[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(lead)}")
+    device = x.device
+    if device != weight.device:
+        raise ValueError(f"x is on {device}, the weight on {weight.device}")
+    lead = lead[:-1]
+    m = lead.numel()
+    rows = (n,)
+    if sections is not None:
+        rows = tuple(int(r) for r in sections)
+        if min(rows, default=0) <= 0 or sum(rows) != n or len(rows) > 8:
+            raise ValueError(f"sections must be 1 to 8 positive row counts that add up to {n}, got {list(rows)}")
+    outs = [torch.empty(lead + (r,), dtype=x.dtype, device=device) for r in rows]
     if m:
         xr, ldx = activation_rows(x)
         seg_rows = (ctypes.c_int * len(rows))(*rows)
         seg_out = (ctypes.c_void_p * len(rows))(*[o.data_ptr() for o in outs])
-        with on_device(x.device):
-            native.call("qm_mx4_linear", native.act_code(x.dtype), m, n, k, native.ptr(weight.codes),
-                        native.ptr(weight.scales), native.ptr(xr), ldx, len(rows), seg_rows, seg_out,
-                        native.stream_handle(x.device))
+        with on_device(device):
+            native.check("qm_mx4_linear", native.load().qm_mx4_linear(
+                act, m, n, k, weight.codes.data_ptr(), weight.scales.data_ptr(), xr.data_ptr(), ldx, len(rows), seg_rows,
+                seg_out, stream_of(device)))
     return outs[0] if sections is None else outs

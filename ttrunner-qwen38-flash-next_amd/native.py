@@ -122,6 +122,8 @@ def load(path: str | None = None) -> ctypes.CDLL:
     """Load the library (once) and bind every entry point; raise if absent.
     The path defaults to QM_LIB from the environment, else the in-tree build."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -145,6 +147,12 @@ def call(name: str, *args) -> int:
         msg = lib.qm_last_error().decode(errors="replace")
         raise QmError(f"{name} failed ({rc}): {msg}")
     return rc
+
+
+def check(name: str, rc: int) -> None:
+    """Raise for a non-zero return code of an entry point called directly."""
+    if rc:
+        raise QmError(f"{name} failed ({rc}): {load().qm_last_error().decode(errors='replace')}")
 
 
 def ptr(t) -> int | None:
