@@ -150,12 +150,12 @@ __global__ __launch_bounds__(64 * FEW) void moe_few_plan_kernel(FewArgs<T> A) {
   }
 }
 
-// h of a slot: a workgroup per 16 hidden units and slot, the waves split k
-template <typename WF, typename T, int PER, bool ONE>
+// h of a slot: a workgroup per 16 TN hidden units and slot, the waves split k
+template <typename WF, typename T, int PER, bool ONE, int TN>
 __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A) {
   using F = Fmt<WF, T>;
   constexpr int NW = FEW_UP_NW, KP = 2;                      // k tiles in flight
-  __shared__ f32x4_t s_red[NW][2][64];
+  __shared__ f32x4_t s_red[NW][2 * TN][64];
   __shared__ int s_id[RT_MAX_TOPK];
   __shared__ float s_w[RT_MAX_TOPK];
   const MoeArgs<T>& M = A.m;
@@ -164,8 +164,10 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
   const int kt = wt_k_tiles(M.hidden), rt = wt_row_tiles(M.inter), slot = blockIdx.y;
   const T* row = M.x + (long)min(r16, M.rows - 1) * M.ldx;
   Acts<F, T> pre[KP];                                        // before it is known which expert
+  if constexpr (ONE) {
 #pragma unroll
-  for (int p = 0; p < KP; ++p) pre[p].load(row, min(wid + p * NW, kt - 1), M.hidden, g4);
+    for (int p = 0; p < KP; ++p) pre[p].load(row, min(wid + p * NW, kt - 1), M.hidden, g4);
+  }
   int e, pair = -1;
   float weight = 0.f;
   if constexpr (ONE) {
@@ -196,34 +198,39 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
   }
   const WMat gate = expert_mat(e < 0 ? M.s_gate : M.gate, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
   const WMat up = expert_mat(e < 0 ? M.s_up : M.up, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
-  f32x4_t acc[2][1];
+  f32x4_t acc[2 * TN][1];
   clear(acc);
   for (int k0 = wid; k0 < kt; k0 += NW * KP) {
-    typename F::W w[KP][2];
+    typename F::W w[KP][2 * TN];
     Acts<F, T> x[KP][1];
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int ks = min(k0 + p * NW, kt - 1);
-      w[p][0] = F::load_w(gate, (long)blockIdx.x * kt + ks, lane);
-      w[p][1] = F::load_w(up, (long)blockIdx.x * kt + ks, lane);
-      if (k0 == wid) x[p][0] = pre[p];
-      else x[p][0].load(row, ks, M.hidden, g4);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) {
+        const long tile = (long)min((int)blockIdx.x * TN + t, rt - 1) * kt + ks;
+        w[p][t] = F::load_w(gate, tile, lane);
+        w[p][TN + t] = F::load_w(up, tile, lane);
+      }
+      // (several tokens: the columns that did not choose the expert load nothing)
+      if (ONE && k0 == wid) x[p][0] = pre[p];
+      else x[p][0].load(row, ks, ONE || pair >= 0 ? M.hidden : 0, g4);
     }
 #pragma unroll
     for (int p = 0; p < KP; ++p)
       if (k0 + p * NW < kt) step_tile<F, T>(acc, w[p], x[p]);
   }
-  s_red[wid][0][lane] = acc[0][0];
-  s_red[wid][1][lane] = acc[1][0];
+#pragma unroll
+  for (int t = 0; t < 2 * TN; ++t) s_red[wid][t][lane] = acc[t][0];
   __syncthreads();
-  if (wid != 0 || pair < 0) return;
-  f32x4_t a = s_red[0][0][lane], b = s_red[0][1][lane];
+  if (wid >= TN || pair < 0) return;
+  f32x4_t a = s_red[0][wid][lane], b = s_red[0][TN + wid][lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) {
-    a += s_red[w][0][lane];
-    b += s_red[w][1][lane];
+    a += s_red[w][wid][lane];
+    b += s_red[w][TN + wid][lane];
   }
-  const int n = blockIdx.x * 16 + 4 * g4;
+  const int n = (blockIdx.x * TN + wid) * 16 + 4 * g4;
   if (n >= M.inter) return;
   f32x4_t v;
 #pragma unroll
@@ -235,7 +242,8 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
 template <typename WF, typename T>
 __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<T> A) {
   using F = Fmt<WF, T>;
-  constexpr int NW = FEW_DOWN_NW, U = 2;
+  // units in flight, as many as 128 registers hold
+  constexpr int NW = FEW_DOWN_NW, U = F::SCALED ? 4 / (int)(sizeof(T) / 2) : sizeof(T) == 2 ? 3 : 1;
   __shared__ f32x4_t s_red[NW][64];
   const MoeArgs<T>& M = A.m;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -243,19 +251,37 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
   const int kt = wt_k_tiles(M.inter), rt = wt_row_tiles(M.hidden);
   const int units = *A.n_slots * kt;
   f32x4_t total = {0.f, 0.f, 0.f, 0.f};
+  // a batch's slots are looked up while the one before is multiplied
+  int expert[U], pair[U], at[U];
+  int slot = wid / kt, ks = wid % kt;                        // of the next unit to look up
+  const int last = units / kt - 1;
+  auto look_up = [&]() {
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      const int s = min(slot, last);
+      expert[p] = A.slot_expert[s];
+      pair[p] = A.slot_pair[s * 16 + r16];
+      at[p] = ks;
+      slot += NW / kt;
+      ks += NW % kt;
+      if (ks >= kt) { ks -= kt; ++slot; }
+    }
+  };
+  look_up();
   for (int u0 = wid; u0 < units; u0 += NW * U) {
     typename F::W w[U][1];
     Acts<F, T> x[U][1];
-    int pair[U];
+    bool mine[U];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int u = min(u0 + p * NW, units - 1), slot = u / kt, ks = u % kt;
-      const int e = A.slot_expert[slot];
-      pair[p] = A.slot_pair[slot * 16 + r16];
+      const int e = expert[p];
       const WMat down = expert_mat(e < 0 ? M.s_down : M.down, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
-      w[p][0] = F::load_w(down, (long)blockIdx.x * kt + ks, lane);
-      x[p][0].load(M.h + (long)max(pair[p], 0) * M.inter, ks, M.inter, g4);
+      w[p][0] = F::load_w(down, (long)blockIdx.x * kt + at[p], lane);
+      // (columns that did not choose the expert load nothing: most of them)
+      mine[p] = pair[p] >= 0;
+      x[p][0].load(M.h + (long)max(pair[p], 0) * M.inter, at[p], mine[p] ? M.inter : 0, g4);
     }
+    look_up();
 #pragma unroll
     for (int p = 0; p < U; ++p) {
       if (u0 + p * NW >= units) continue;
@@ -264,7 +290,7 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
       step_tile<F, T>(acc, w[p], x[p]);
       // a token that did not choose the expert takes nothing from it, whatever it is
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total[i] += pair[p] < 0 ? 0.f : acc[0][0][i];
+      for (int i = 0; i < 4; ++i) total[i] += mine[p] ? acc[0][0][i] : 0.f;
     }
   }
   s_red[wid][lane] = total;
@@ -301,14 +327,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void moe_up_gemm_kernel(MoeArgs<T>
   const WMat gate = expert_mat(R.is_shared ? A.s_gate : A.gate, R.e, (long)rt * kt, G::F::TILE);
   const WMat up = expert_mat(R.is_shared ? A.s_up : A.up, R.e, (long)rt * kt, G::F::TILE);
   auto first = [&](int q) { return (long)min(t0 + q / TN * HN + q % HN, rt - 1) * kt; };
-  const typename G::Src src = G::source(
-      wid, lane,
-      [&](int i) { return A.x + (long)(pair_of(R, min(tile.y + i, R.count - 1), A.ppt) / A.ppt) * A.ldx; },
-      [&](int q) { return static_cast<const char*>(q % TN < HN ? gate.data : up.data) + first(q) * G::F::TILE; },
-      [&](int q) { return (q % TN < HN ? gate.scales : up.scales) + first(q) * 64; });
+  auto row = [&](int i) { return A.x + (long)(pair_of(R, min(tile.y + i, R.count - 1), A.ppt) / A.ppt) * A.ldx; };
+  auto weight = [&](int q) { return static_cast<const char*>(q % TN < HN ? gate.data : up.data) + first(q) * G::F::TILE; };
+  const typename G::Src src =
+      G::source(wid, lane, row, weight, [&](int q) { return (q % TN < HN ? gate.scales : up.scales) + first(q) * 64; });
   f32x4_t acc[TN][TM];
   clear(acc);
-  G::run(acc, s_buf, src, A.hidden);
+  G::run(acc, s_buf, src, A.hidden, R.count - tile.y);
 #pragma unroll
   for (int u = 0; u < TM; ++u) {
     const int m = tile.y + (wid % WM) * 16 * TM + 16 * u + (lane & 15);
@@ -341,13 +366,12 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void moe_down_gemm_kernel(MoeArgs<
   const int t0 = item % nt * WN * TN;
   const WMat down = expert_mat(R.is_shared ? A.s_down : A.down, R.e, (long)rt * kt, G::F::TILE);
   auto first = [&](int q) { return (long)min(t0 + q, rt - 1) * kt; };
-  const typename G::Src src = G::source(
-      wid, lane, [&](int i) { return A.h + (long)pair_of(R, min(tile.y + i, R.count - 1), A.ppt) * A.inter; },
-      [&](int q) { return static_cast<const char*>(down.data) + first(q) * G::F::TILE; },
-      [&](int q) { return down.scales + first(q) * 64; });
+  auto row = [&](int i) { return A.h + (long)pair_of(R, min(tile.y + i, R.count - 1), A.ppt) * A.inter; };
+  auto weight = [&](int q) { return static_cast<const char*>(down.data) + first(q) * G::F::TILE; };
+  const typename G::Src src = G::source(wid, lane, row, weight, [&](int q) { return down.scales + first(q) * 64; });
   f32x4_t acc[TN][TM];
   clear(acc);
-  G::run(acc, s_buf, src, A.inter);
+  G::run(acc, s_buf, src, A.inter, R.count - tile.y);
 #pragma unroll
   for (int u = 0; u < TM; ++u) {
     const int m = tile.y + (wid % WM) * 16 * TM + 16 * u + (lane & 15);
@@ -413,24 +437,21 @@ struct MoeLayout {
 };
 
 // Activation rows of a tile of the many-token kernels, by the rows that an expert
-// has on average (us a layer of 128 experts of 2048 x 512, 8 of them chosen, bf16;
-// tiles of 16 / 32 / 64 / 128 rows, the best width of each):
-//   bf16 weights    8 rows 175 / 174 / 178 / 183, 25 rows 227 / 196 / 197 / 203, 62
-//                   rows 347 / 264 / 234 / 245, 250 rows of 64 wider experts 816 /
-//                   503 / 343 / 322
-//   4-bit weights   8 rows 84 / 80 / 99 / 160, 62 rows 187 / 142 / 153 / 200, 250
-//                   rows 376 / 251 / 251 / 271
-//   float           12 rows of bf16 weights' place taken by float ones 170 / 170 /
-//                   301; with 4-bit ones 25 rows 127 / 142 / 308
-struct TileRule {
-  int rows;
-};
-TileRule tile_rule(const qm_moe_geom& g) {
+// has on average (us a layer, 8 experts of a token; tiles of 16 / 32 / 64 / 128
+// rows, the best shape of each):
+//   bf16 weights, 128 experts of 2048 x 512: 8 rows 175 / 174 / 178 / 183, 25 rows
+//     227 / 196 / 197 / 203, 62 rows 347 / 264 / 234 / 245; 64 of 2048 x 768: 250
+//     rows 806 / 464 / 343 / 322
+//   4-bit weights: 8 rows 84 / 79 / 98 / 182, 31 rows - / 118 / 122 / 205, 125 rows
+//     - / 231 / 236 / 303, 750 rows (2048 x 768) - / 742 / 710 / 897
+//   float activations, 25 rows: float weights 340 / 231 / 376, 4-bit ones 127 / 142
+//     / 308
+int rows_per_tile(const qm_moe_geom& g) {
   const double avg = (double)g.rows * g.top_k / g.experts;
   const bool mx = g.weight_format == QM_W_MX4;
-  if (g.act_dtype != QM_ACT_BF16) return {mx ? 16 : 32};
-  if (mx) return {avg < 256 ? 32 : 64};
-  return {avg < 40 ? 32 : avg < 128 ? 64 : 128};
+  if (g.act_dtype != QM_ACT_BF16) return mx ? 16 : 32;
+  if (mx) return avg < 512 ? 32 : 64;
+  return avg < 40 ? 32 : avg < 128 ? 64 : 128;
 }
 // The few-token kernels take the table of slots where the others keep the lists.
 MoeLayout moe_layout(const qm_moe_geom& g) {
@@ -448,7 +469,7 @@ MoeLayout moe_layout(const qm_moe_geom& g) {
     l.lists = take((g.shared + hot) * 16 * sizeof(int));      // slot_pair
     l.pair_w = take((g.shared + hot) * 16 * sizeof(float));   // slot_w
   } else {
-    l.bm = tile_rule(g).rows;
+    l.bm = rows_per_tile(g);
     // every expert's last tile may be part-filled
     l.max_tiles = (long)(choices / l.bm + hot + g.shared * ((t + l.bm - 1) / l.bm));
     l.norms = take(qm_route_norms(g.experts));
@@ -502,29 +523,31 @@ int launch_gemms(const MoeArgs<T>& A, long max_tiles, hipStream_t stream) {
 
 template <typename WF, typename T>
 int launch_ffn(const MoeArgs<T>& A, int bm, long max_tiles, hipStream_t stream) {
-  // (tile_rule)
   if constexpr (sizeof(T) == 4) {
     if constexpr (Fmt<WF, T>::SCALED) return launch_gemms<WF, T, 4, 1, 2, 1, 2>(A, max_tiles, stream);
     else return launch_gemms<WF, T, 2, 2, 4, 1, 2>(A, max_tiles, stream);
   } else if constexpr (Fmt<WF, T>::SCALED) {
-    return bm == 32 ? launch_gemms<WF, T, 4, 2, 4, 1, 2>(A, max_tiles, stream)
-                    : launch_gemms<WF, T, 2, 4, 4, 1, 2>(A, max_tiles, stream);
+    return bm == 32 ? launch_gemms<WF, T, 2, 2, 8, 1, 2>(A, max_tiles, stream)
+                    : launch_gemms<WF, T, 4, 2, 4, 2, 2>(A, max_tiles, stream);
   } else {
     if (bm == 32) return launch_gemms<WF, T, 2, 2, 4, 1, 3>(A, max_tiles, stream);
     return bm == 64 ? launch_gemms<WF, T, 2, 4, 4, 1, 3>(A, max_tiles, stream)
-                    : launch_gemms<WF, T, 4, 4, 2, 2, 2>(A, max_tiles, stream);
+                    : launch_gemms<WF, T, 2, 4, 4, 2, 2>(A, max_tiles, stream);
   }
 }
 
 template <typename WF, typename T, int PER>
 int launch_few_per(const FewArgs<T>& A, int max_slots, hipStream_t stream) {
-  const dim3 up(wt_row_tiles(A.m.inter), max_slots);
+  // 4-bit weights are few bytes beside the activations' operands: two tiles share them
+  constexpr int TN = Fmt<WF, T>::SCALED ? 2 : 1;
+  const int rt = wt_row_tiles(A.m.inter);
   if (A.m.rows == 1) {
-    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, PER, true>), up, dim3(64 * FEW_UP_NW), 0, stream, A);
+    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, PER, true, 1>), dim3(rt, max_slots), dim3(64 * FEW_UP_NW), 0, stream, A);
   } else {
     hipLaunchKernelGGL((moe_few_plan_kernel<T, PER>), dim3(1), dim3(64 * FEW), 0, stream, A);
     QM_CHECK_LAUNCH();
-    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, 1, false>), up, dim3(64 * FEW_UP_NW), 0, stream, A);
+    hipLaunchKernelGGL((moe_few_up_kernel<WF, T, 1, false, TN>), dim3((rt + TN - 1) / TN, max_slots), dim3(64 * FEW_UP_NW), 0,
+                       stream, A);
   }
   QM_CHECK_LAUNCH();
   hipLaunchKernelGGL((moe_few_down_kernel<WF, T>), dim3(wt_row_tiles(A.m.hidden)), dim3(64 * FEW_DOWN_NW), 0, stream, A);

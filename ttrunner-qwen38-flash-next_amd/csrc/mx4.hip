@@ -96,34 +96,43 @@ __global__ __launch_bounds__(MX_NT) void mx4_quantize_kernel(MxGeom g, const T* 
   scales[tile * 64 + lane] = (uint8_t)s;
 }
 
-__device__ __forceinline__ void store32(bf16_t* p, const u32x4_t& q, float scale) {
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-    *reinterpret_cast<uint4*>(p + 8 * d) = __builtin_bit_cast(uint4, mx4_frag(q[d], scale));
-}
-__device__ __forceinline__ void store32(float* p, const u32x4_t& q, float scale) {
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 0);
-    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 1);
-    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 2);
-    const auto e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[d], scale, 3);
-    *reinterpret_cast<float4*>(p + 8 * d) = make_float4(a[0], a[1], b[0], b[1]);
-    *reinterpret_cast<float4*>(p + 8 * d + 4) = make_float4(c[0], c[1], e[0], e[1]);
-  }
-}
-
+// A lane writes 16 bytes of the output, 256 or 512 contiguous bytes a row (a lane
+// per block, 64 or 128 bytes apart, wrote 52 M bf16 weights at 3.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(MX_NT) void mx4_dequantize_kernel(MxGeom g, const uint8_t* codes, const uint8_t* scales,
                                                               T* out) {
+  constexpr int VE = 16 / sizeof(T), UNITS = WT_K / VE, RPS = 64 / UNITS;   // rows of one wave-wide store
   const int lane = threadIdx.x & 63;
   const long tile = (long)blockIdx.x * (MX_NT / 64) + (threadIdx.x >> 6);
   if (tile >= g.tiles) return;
-  long row;
-  int k0;
-  if (!block_of(g, tile, lane, row, k0)) return;
-  const u32x4_t q = *reinterpret_cast<const u32x4_t*>(codes + tile * 1024 + lane * 16);
-  store32(out + row * g.k + k0, q, __uint_as_float((unsigned)scales[tile * 64 + lane] << 23));
+  const int ks = (int)(tile % g.kt);
+  const long rest = tile / g.kt;
+  const int u = lane % UNITS, k0 = ks * WT_K + u * VE, g4 = u * VE / MX_BLOCK;
+  const int r0 = (int)(rest % g.rt) * WT_ROWS;
+  unsigned q[WT_ROWS / RPS];
+  unsigned char s[WT_ROWS / RPS];
+#pragma unroll
+  for (int i = 0; i < WT_ROWS / RPS; ++i) {
+    const int slot = g4 * 16 + i * RPS + lane / UNITS;
+    // the dword with this unit's codes: 8 of them (all of it, or a half)
+    q[i] = *reinterpret_cast<const unsigned*>(codes + tile * 1024 + slot * 16 + u * VE % MX_BLOCK / 8 * 4);
+    s[i] = scales[tile * 64 + slot];
+  }
+#pragma unroll
+  for (int i = 0; i < WT_ROWS / RPS; ++i) {
+    const int r = r0 + i * RPS + lane / UNITS;
+    if (r >= g.n || k0 >= g.k) continue;
+    const float scale = __uint_as_float((unsigned)s[i] << 23);
+    T* p = out + (rest / g.rt * g.n + r) * g.k + k0;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, mx4_frag(q[i], scale));
+    } else {
+      const unsigned h = u & 1 ? q[i] >> 16 : q[i];
+      const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(h, scale, 0);
+      const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(h, scale, 1);
+      *reinterpret_cast<float4*>(p) = make_float4(a[0], a[1], b[0], b[1]);
+    }
+  }
 }
 
 // between the plain order (codes [rows, k / 2], scales [rows, k / 32]) and tiles
@@ -245,7 +254,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void mx4_gemm_kernel(Mx4LinearArgs
       [&](int q) { return A.w.scales + first(q) * 64; });
   f32x4_t acc[TN][TM];
   clear(acc);
-  G::run(acc, s_buf, src, A.k);
+  G::run(acc, s_buf, src, A.k, A.m - m0);
 #pragma unroll
   for (int t = 0; t < TN; ++t)
 #pragma unroll
@@ -272,8 +281,8 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
 //     with two tiles 4.5 and 6.4)
 //   bf16, more rows   the largest of the tiles of wgemm.h that makes 256 workgroups
 //     (160 for the smallest). 12352 x 2048, 256 x 64 / 256 x 32 / 128 x 32 / 128 x 16
-//     tiles: 64 rows 26 / 16.6 / 11.7 / 10.6, 128 rows 26 / 16.8 / 13.8 / 18.1, 256
-//     rows 26 / 22.0 / 25.6 / 26.8, 512 rows 34.6 / 40.2 / 39.8 / 50. Fewer
+//     tiles: 64 rows 20.2 / 13.9 / 11.7 / 10.6, 128 rows 20.5 / 14.4 / 13.8 / 18.1,
+//     256 rows 21.2 / 20.1 / 25.6 / 26.8, 512 rows 33.1 / 37.3 / 39.8 / 50. Fewer
 //     workgroups than that: the few-row kernel with k split over 16 waves (2048 x
 //     4096: 64 rows 7.1 against 14.4, 128 rows 12.1 against 14.5)
 //   float   the same with the smallest tile alone (its activations are cut into
@@ -287,8 +296,8 @@ int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
     return launch_rows<T, 1, 1, 8, 2>(A, stream);
   }
   if constexpr (sizeof(T) == 2) {
-    if (groups(256, 64) >= 256) return launch_gemm<T, 4, 4, 4, 1, 2>(A, stream);
-    if (groups(256, 32) >= 256) return launch_gemm<T, 4, 2, 4, 1, 2>(A, stream);
+    if (groups(256, 64) >= 256) return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
+    if (groups(256, 32) >= 256) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
     if (groups(128, 32) >= 256) return launch_gemm<T, 2, 2, 4, 1, 3>(A, stream);
     if (groups(128, 16) >= 160) return launch_gemm<T, 2, 1, 4, 1, 4>(A, stream);
     return launch_rows<T, 2, 1, 16, 1>(A, stream);

@@ -21,6 +21,11 @@
 namespace {
 
 constexpr double ROUTE_FEW = 1e8;
+// Choices of an expert, on average, up to which the choosing waves file them by
+// atomics (they serialise: 8 each +2.4 us, 16 +4.2, 32 +7.2, 250 +31); beyond, a
+// launch of its own does (6.0 us and its start, 7.7 at 16000 choices)
+constexpr int LISTS_ATOMIC = 24;
+
 constexpr int RT_TB = 4;                 // token rows of one wave of the few-row logits
 
 // 16 bytes as floats
@@ -241,8 +246,9 @@ __device__ __forceinline__ double exact_logit(const QmLogits<T>& A, int t, int e
 
 // The workgroup that finishes last makes the table of row tiles from the counts,
 // the shared experts first.
+template <int NT>
 __device__ __forceinline__ void finish_lists(int rows, int experts, const QmRouteLists& L) {
-  __shared__ int s_wave[4];
+  __shared__ int s_wave[NT / 64];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   wait_all_memory();                                         // this wave's counts are in
@@ -253,7 +259,7 @@ __device__ __forceinline__ void finish_lists(int rows, int experts, const QmRout
   if (!s_last) return;
   int start = 0;
   const int all = L.shared + experts;
-  for (int y0 = 0; y0 < all; y0 += 256) {
+  for (int y0 = 0; y0 < all; y0 += NT) {
     const int y = y0 + threadIdx.x;
     int count = 0;
     if (y < all) count = y < L.shared ? rows : (int)ld_flag(reinterpret_cast<const unsigned*>(L.counts + y - L.shared));
@@ -269,7 +275,7 @@ __device__ __forceinline__ void finish_lists(int rows, int experts, const QmRout
     __syncthreads();
     int place = start + before - mine;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
       const int c = s_wave[w];
       if (w < wid) place += c;
       start += c;
@@ -277,6 +283,55 @@ __device__ __forceinline__ void finish_lists(int rows, int experts, const QmRout
     for (int i = 0; i < mine; ++i) L.tiles[place + i] = make_int2(y, i * L.bm);
   }
   if (threadIdx.x == 0) *L.n_tiles = start;
+}
+
+// The lists of many choices, a workgroup per expert: a thread finds the hits among
+// 16 consecutive choices, a scan over the workgroup places them.
+constexpr int LS_NT = 1024, LS_PER = 16;
+__global__ __launch_bounds__(LS_NT) void moe_lists_kernel(const int* ids, int rows, int top_k, QmRouteLists L) {
+  __shared__ int s_hits[LS_NT / 64];
+  const int e = blockIdx.x, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int n = rows * top_k;
+  int* list = L.lists + (long)e * rows;
+  int at = 0;
+  for (int p0 = 0; p0 < n; p0 += LS_NT * LS_PER) {
+    const int p = p0 + threadIdx.x * LS_PER;
+    unsigned hits = 0;
+    if (p + LS_PER <= n) {                                   // ids are 16-byte aligned
+#pragma unroll
+      for (int i = 0; i < LS_PER / 4; ++i) {
+        const int4 v = *reinterpret_cast<const int4*>(ids + p + 4 * i);
+        hits |= ((v.x == e) | (v.y == e) << 1 | (v.z == e) << 2 | (v.w == e) << 3) << (4 * i);
+      }
+    } else {
+      for (int i = 0; i < LS_PER; ++i)
+        if (p + i < n && ids[p + i] == e) hits |= 1u << i;
+    }
+    const int mine = __popc(hits);
+    int before = mine;                                       // inclusive scan over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(before, d, 64);
+      if (lane >= d) before += o;
+    }
+    if (lane == 63) s_hits[wid] = before;
+    __syncthreads();
+    int place = at + before - mine;
+#pragma unroll
+    for (int w = 0; w < LS_NT / 64; ++w) {
+      const int c = s_hits[w];
+      if (w < wid) place += c;
+      at += c;
+    }
+    while (hits) {
+      const int q = p + __ffs(hits) - 1;
+      list[place++] = q / top_k * L.ppt + q % top_k;
+      hits &= hits - 1;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) st_flag(reinterpret_cast<unsigned*>(L.counts + e), (unsigned)at);
+  finish_lists<LS_NT>(rows, gridDim.x, L);
 }
 
 // A token's choice, by one wave
@@ -417,7 +472,7 @@ __global__ __launch_bounds__(256) void moe_topk_kernel(QmLogits<T> A, TopArgs P)
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t < A.rows) topk_row<T, PER>(A, P, t, lane);
-  if (P.lists.counts) finish_lists(A.rows, A.experts, P.lists);
+  if (P.lists.counts) finish_lists<256>(A.rows, A.experts, P.lists);
 }
 
 template <typename T, int PER>
@@ -456,11 +511,17 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
     QM_CHECK_LAUNCH();
   }
   if (rc) return rc;
-  if (A.experts <= 64) return launch_topk<T, 1>(A, P, stream);
-  if (A.experts <= 128) return launch_topk<T, 2>(A, P, stream);
-  if (A.experts <= 256) return launch_topk<T, 4>(A, P, stream);
-  if (A.experts <= 512) return launch_topk<T, 8>(A, P, stream);
-  return launch_topk<T, 16>(A, P, stream);
+  const bool apart = lists && (long)A.rows * top_k > (long)LISTS_ATOMIC * A.experts;
+  if (apart) P.lists = QmRouteLists{};
+  if (A.experts <= 64) rc = launch_topk<T, 1>(A, P, stream);
+  else if (A.experts <= 128) rc = launch_topk<T, 2>(A, P, stream);
+  else if (A.experts <= 256) rc = launch_topk<T, 4>(A, P, stream);
+  else if (A.experts <= 512) rc = launch_topk<T, 8>(A, P, stream);
+  else rc = launch_topk<T, 16>(A, P, stream);
+  if (rc || !apart) return rc;
+  hipLaunchKernelGGL(moe_lists_kernel, dim3(A.experts), dim3(LS_NT), 0, stream, ids, A.rows, top_k, *lists);
+  QM_CHECK_LAUNCH();
+  return QM_OK;
 }
 
 template int qm_route_logits<bf16_t>(const QmLogits<bf16_t>&, hipStream_t);

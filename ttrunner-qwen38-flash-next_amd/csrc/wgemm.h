@@ -27,7 +27,7 @@ struct SpanGemm {
   static constexpr int RPL = 1024 / ROW_B;                     // rows of one wave-wide load
   static constexpr int XL = BM / RPL / NW;                     // activation loads of a wave, per span
   static constexpr int WL = TN * WN * F::SPAN_B / 1024 / NW;   // weight loads
-  static constexpr int LOADS = XL + WL + (F::SCALED ? 1 : 0);
+  static constexpr int W_LOADS = WL + (F::SCALED ? 1 : 0);
   static constexpr int X_B = BM * ROW_B, W_B = TN * WN * F::SPAN_B, S_B = F::SCALED ? NW * 256 : 0;
   static constexpr int BUF = X_B + W_B + S_B, LDS_BYTES = S * BUF;
   static_assert(XL * RPL * NW == BM && WL * 1024 * NW == W_B && TN <= 4 && XL > 0 && WL > 0, "loads of a wave");
@@ -56,41 +56,42 @@ struct SpanGemm {
   }
   __device__ __forceinline__ static int swizzle(int row) { return UNITS >= 16 ? row & 15 : row >> 1 & 7; }
 
-  __device__ __forceinline__ static void fetch(char* buf, const Src& src, int k, int j, int wid, int lane) {
+  __device__ __forceinline__ static void fetch(char* buf, const Src& src, int k, int rows, int j, int wid, int lane) {
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-      const int at = (wid * XL + i) * 1024;
-      const int unit = (lane % UNITS) ^ swizzle((wid * XL + i) * RPL + lane / UNITS);
+      const int at = (wid * XL + i) * 1024, row = (wid * XL + i) * RPL + lane / UNITS;
+      const int unit = (lane % UNITS) ^ swizzle(row);
       // units past k (a last span that is partly past it) are zeros: whatever lies
       // behind a row would meet weights of zero, but infinities make NaN of those
       const int kk = j * F::SPAN + unit * VE;
       const void* p = kk < k ? static_cast<const void*>(src.x[i] + kk) : g_zero_unit;
-      lds_load16(p, buf + at);
+      if (row < rows) lds_load16(p, buf + at);                // (rows past the last multiply what lies there, unread)
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) lds_load16(src.w[i] + (long)j * F::SPAN_B, buf + X_B + (wid * WL + i) * 1024);
     if constexpr (F::SCALED) lds_load4(src.s + (long)j * 64, buf + X_B + W_B + wid * 256);
   }
-  __device__ __forceinline__ static void run(f32x4_t (&acc)[TN][TM], char* lds, const Src& src, int k) {
+  __device__ __forceinline__ static void run(f32x4_t (&acc)[TN][TM], char* lds, const Src& src, int k, int rows) {
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = lane >> 4, row0 = (wid % WM) * 16 * TM + (lane & 15), wn = wid / WM;
     const int spans = (k + F::SPAN - 1) / F::SPAN;
 #pragma unroll
     for (int j = 0; j < S - 1; ++j)
-      if (j < spans) fetch(lds + j * BUF, src, k, j, wid, lane);
+      if (j < spans) fetch(lds + j * BUF, src, k, rows, j, wid, lane);
     for (int j0 = 0; j0 < spans; j0 += S) {
 #pragma unroll
       for (int b = 0; b < S; ++b) {
         const int j = j0 + b;
         if (j >= spans) break;
         // this wave's part of span j is in LDS when at most the S - 2 later
-        // spans' loads are outstanding (loads return in order), its reads of the
-        // buffer that is filled next when none of LDS is
+        // spans' loads are outstanding (loads return in order; those of
+        // activations do not count, a wave whose rows lie past the last makes
+        // none), its reads of the buffer that is filled next when none of LDS is
         if (j + S - 2 < spans)
-          wave_loads_barrier<(S - 2) * LOADS>();
+          wave_loads_barrier<(S - 2) * W_LOADS>();
         else
           wave_loads_barrier<0>();
-        if (j + S - 1 < spans) fetch(lds + (b + S - 1) % S * BUF, src, k, j + S - 1, wid, lane);
+        if (j + S - 1 < spans) fetch(lds + (b + S - 1) % S * BUF, src, k, rows, j + S - 1, wid, lane);
         const char* buf = lds + b * BUF;
         typename F::W w[TN];
 #pragma unroll
@@ -121,6 +122,4 @@ struct SpanGemm {
       }
     }
   }
-
-  static_assert((S - 2) * LOADS < 64, "vmcnt has 6 bits");
 };
