@@ -2,7 +2,8 @@
 
 Same field names and derivations as the reference config
 (reference/config.py:51-52, 80-104, 136-158), restricted to what QSA, Gated
-DeltaNet and the hyper-connections around them read, plus the paging
+DeltaNet, the hyper-connections around them and the mixture of experts read
+(the experts' number and widths come from their weights), plus the paging
 parameters this implementation adds (``page_size``).
 ``from_reference`` accepts any object carrying the reference's field names
 (a ``Qwen4ExpConfig`` or a test double), so the layers drop into the reference
@@ -36,6 +37,9 @@ class MixConfig:
     output_gate_type: str = "sigmoid"
     hc_count: int = 4
     hc_lowrank: int = 320
+    num_experts_per_tok: int = 8
+    norm_topk_prob: bool = True
+    shared_expert: bool = True
     page_size: int = 64
 
     @property

@@ -1,5 +1,5 @@
-"""The token-mixing half of a decode step over a stack of layers, replayable
-from one HIP graph.
+"""The token-mixing half of a decode step over a stack of layers (with
+``ffn=True`` the layers' experts too), replayable from one HIP graph.
 
 For one token per sequence, ``MixDecoder`` runs the attention half of every
 decoder layer of the reference's forward pass (reference/model.py:443-452):
@@ -52,10 +52,61 @@ from . import native
 from .plan import DnDecodePlan, QsaDecodePlan
 
 
-class _LayerStep:
-    """One layer's token-mixing half for B rows, every buffer bound."""
+def _project(entry, act, rows, x, w, sizes, outs, seg_rows, seg_out, stream):
+    """outs = the projections of x [rows, K] by w: in one launch of ``entry``, or
+    by library GEMMs where that is None."""
+    if entry == "qm_mx4_linear":
+        n, k = w.shape
+        native.call(entry, act, rows, n, k, w.codes.data_ptr(), w.scales.data_ptr(), x.data_ptr(), k, len(sizes),
+                    seg_rows, seg_out, stream)
+        return
+    if entry:
+        native.call(entry, act, rows, int(w.shape[0]), int(w.shape[1]), w.data_ptr(), x.data_ptr(), len(sizes),
+                    seg_rows, seg_out, stream)
+        return
+    x2 = x.view(rows, -1)
+    start = 0
+    for r, o in zip(sizes, outs):
+        torch.matmul(x2, w[start:start + r].t(), out=o.view(rows, r))
+        start += r
 
-    def __init__(self, model, cache, layer: int, max_position: int, positions: torch.Tensor, dtype):
+
+class _FfnStep:
+    """One layer's mixture-of-experts half for ``rows`` token rows, every buffer
+    bound: the hyper-connection mix (by the kernels of ``as_rows`` rows), the
+    experts, and the reinjection into the residual."""
+
+    def __init__(self, model, layer: int, rows: int, as_rows: int, dtype):
+        c = model.config
+        dev = model.device
+        lib = native.load()
+        self.as_rows = as_rows
+        self.norm_w, self.w_di, self.w_up, _ = model.hc_weights(layer, "ffn", dtype)
+        self.hc_geom = model.hc_geom(rows, dtype)
+        self.hc_ws = torch.zeros(lib.qm_hc_mix_workspace(ctypes.byref(self.hc_geom)), dtype=torch.uint8, device=dev)
+        self.ri_geom = native.HcGeom(rows, c.hc_count, c.hidden_size, 0, native.act_code(dtype), 0.0)
+        self.mixed = torch.empty(rows, c.hidden_size, dtype=dtype, device=dev)
+        self.inject = torch.empty(rows, c.hc_count, dtype=dtype, device=dev)
+        self.branch = torch.empty(rows, c.hidden_size, dtype=dtype, device=dev)
+        self.weights = model.moe_weights(layer, dtype)
+        self.geom = self.weights.geom(rows)
+        self.ws = torch.empty(lib.qm_moe_workspace(ctypes.byref(self.geom)), dtype=torch.uint8, device=dev)
+
+    def launch(self, hyper: torch.Tensor, stream: int):
+        native.call("qm_hc_mix_as", ctypes.byref(self.hc_geom), self.as_rows, hyper.data_ptr(), self.norm_w.data_ptr(),
+                    self.w_di.data_ptr(), 1, self.w_up.data_ptr(), self.mixed.data_ptr(), self.inject.data_ptr(),
+                    self.hc_ws.data_ptr(), self.hc_ws.numel(), stream)
+        native.call("qm_moe", ctypes.byref(self.geom), ctypes.byref(self.weights.ptrs), self.mixed.data_ptr(),
+                    self.mixed.shape[1], self.branch.data_ptr(), self.ws.data_ptr(), self.ws.numel(), stream)
+        native.call("qm_hc_reinject", ctypes.byref(self.ri_geom), hyper.data_ptr(), self.branch.data_ptr(),
+                    self.inject.data_ptr(), hyper.data_ptr(), stream)
+
+
+class _LayerStep:
+    """One layer's token-mixing half for B rows, every buffer bound (and its
+    experts' half, where the decoder runs that too)."""
+
+    def __init__(self, model, cache, layer: int, max_position: int, positions: torch.Tensor, dtype, ffn: bool = False):
         c = model.config
         B = cache.batch
         dev = model.device
@@ -75,8 +126,8 @@ class _LayerStep:
         self.hc = c.hc_count
         # projections
         g_in, g_out = ("qsa_in", "qsa_out") if self.is_qsa else ("dn_in", "dn_out")
-        self.w_in, rows_in = model._wcat(layer, g_in, dtype)
-        self.w_out, rows_out = model._wcat(layer, g_out, dtype)
+        self.w_in, rows_in = model.proj_weights(layer, g_in, dtype)
+        self.w_out, rows_out = model.proj_weights(layer, g_out, dtype)
         self.ins = [torch.empty(B, 1, r, dtype=dtype, device=dev) for r in rows_in]
         self.branch = torch.empty(B, 1, rows_out[0], dtype=dtype, device=dev)
         self.rows_in, self.rows_out = rows_in, rows_out
@@ -92,19 +143,17 @@ class _LayerStep:
         else:
             self.core = DnDecodePlan(model, cache, layer, dtype)
         self.core.positions = positions
+        self.ffn = _FfnStep(model, layer, B, B, dtype) if ffn else None
 
     def _project(self, x, w, rows, outs, seg_rows, seg_out, entry, stream):
-        if entry:
-            native.call(entry, self.act, self.rows, int(w.shape[0]), int(w.shape[1]), w.data_ptr(),
-                        x.data_ptr(), len(rows), seg_rows, seg_out, stream)
-            return
-        x2 = x.view(self.rows, -1)
-        start = 0
-        for r, o in zip(rows, outs):
-            torch.matmul(x2, w[start:start + r].t(), out=o.view(self.rows, r))
-            start += r
+        _project(entry, self.act, self.rows, x, w, rows, outs, seg_rows, seg_out, stream)
 
     def launch(self, hyper: torch.Tensor, stream: int):
+        self._launch_mixing(hyper, stream)
+        if self.ffn is not None:
+            self.ffn.launch(hyper, stream)
+
+    def _launch_mixing(self, hyper: torch.Tensor, stream: int):
         native.call("qm_hc_mix", ctypes.byref(self.hc_geom), hyper.data_ptr(), self.norm_w.data_ptr(),
                     self.w_di.data_ptr(), 1, self.w_up.data_ptr(), self.mixed.data_ptr(), self.inject.data_ptr(),
                     self.hc_ws.data_ptr(), self.hc_ws.numel(), stream)
@@ -115,13 +164,13 @@ class _LayerStep:
         else:
             qkv, z, b, a = self.ins
             out = self.core.run(qkv, z, a, b, stream)
-        if self.proj_out:
+        if self.proj_out not in (None, "qm_mx4_linear"):
             # the output projection with the reinjection as its epilogue
             native.call(self.proj_out + "_reinject", self.act, self.rows, self.rows_out[0], int(self.w_out.shape[1]),
                         self.w_out.data_ptr(), out.data_ptr(), self.hc, self.inject.data_ptr(), hyper.data_ptr(),
                         stream)
             return
-        self._project(out, self.w_out, self.rows_out, [self.branch], self._seg_out, self._out_out, None, stream)
+        self._project(out, self.w_out, self.rows_out, [self.branch], self._seg_out, self._out_out, self.proj_out, stream)
         native.call("qm_hc_reinject", ctypes.byref(self.ri_geom), hyper.data_ptr(), self.branch.data_ptr(),
                     self.inject.data_ptr(), hyper.data_ptr(), stream)
 
@@ -148,7 +197,7 @@ class _LayerStepN:
     as the layer methods that MixDecoder.step_n calls, so a replay equals that
     eager pass bit for bit."""
 
-    def __init__(self, model, cache, layer: int, k: int, positions: torch.Tensor, dtype):
+    def __init__(self, model, cache, layer: int, k: int, positions: torch.Tensor, dtype, ffn: bool = False):
         c = model.config
         dev = model.device
         lib = native.load()
@@ -168,8 +217,8 @@ class _LayerStepN:
         self.hc = c.hc_count
         # projections
         g_in, g_out = ("qsa_in", "qsa_out") if self.is_qsa else ("dn_in", "dn_out")
-        self.w_in, self.rows_in = model._wcat(layer, g_in, dtype)
-        self.w_out, self.rows_out = model._wcat(layer, g_out, dtype)
+        self.w_in, self.rows_in = model.proj_weights(layer, g_in, dtype)
+        self.w_out, self.rows_out = model.proj_weights(layer, g_out, dtype)
         self.ins = [torch.empty(1, k, r, dtype=dtype, device=dev) for r in self.rows_in]
         self.branch = torch.empty(1, k, self.rows_out[0], dtype=dtype, device=dev)
         self.proj_in = model._proj_entry(dtype, k, c.hidden_size, len(self.rows_in))
@@ -204,19 +253,17 @@ class _LayerStepN:
                                                               ("ssm_conv1d.weight", dtype),
                                                               ("ssm_norm.weight", torch.float32))}
             self.out = torch.empty(1, k, c.linear_value_dim, dtype=dtype, device=dev)
+        self.ffn = _FfnStep(model, layer, k, _mix_as_rows(1, k), dtype) if ffn else None
 
     def _project(self, x, w, rows, outs, seg_rows, seg_out, entry, stream):
-        if entry:
-            native.call(entry, self.act, self.k, int(w.shape[0]), int(w.shape[1]), w.data_ptr(),
-                        x.data_ptr(), len(rows), seg_rows, seg_out, stream)
-            return
-        x2 = x.view(self.k, -1)
-        start = 0
-        for r, o in zip(rows, outs):
-            torch.matmul(x2, w[start:start + r].t(), out=o.view(self.k, r))
-            start += r
+        _project(entry, self.act, self.k, x, w, rows, outs, seg_rows, seg_out, stream)
 
     def launch(self, hyper: torch.Tensor, stream: int):
+        self._launch_mixing(hyper, stream)
+        if self.ffn is not None:
+            self.ffn.launch(hyper, stream)
+
+    def _launch_mixing(self, hyper: torch.Tensor, stream: int):
         native.call("qm_hc_mix_as", ctypes.byref(self.hc_geom), _mix_as_rows(1, self.k), hyper.data_ptr(),
                     self.norm_w.data_ptr(), self.w_di.data_ptr(), 1, self.w_up.data_ptr(), self.mixed.data_ptr(),
                     self.inject.data_ptr(), self.hc_ws.data_ptr(), self.hc_ws.numel(), stream)
@@ -244,12 +291,12 @@ class _LayerStepN:
                         w["ssm_conv1d.weight"].data_ptr(), w["ssm_norm.weight"].data_ptr(), pos,
                         lc.conv_ring.data_ptr(), lc.recurrent_state.data_ptr(), self.out.data_ptr(),
                         self.ws.data_ptr(), self.ws.numel(), stream)
-        if self.proj_out:
+        if self.proj_out not in (None, "qm_mx4_linear"):
             native.call(self.proj_out + "_reinject", self.act, self.k, self.rows_out[0], int(self.w_out.shape[1]),
                         self.w_out.data_ptr(), self.out.data_ptr(), self.hc, self.inject.data_ptr(),
                         hyper.data_ptr(), stream)
             return
-        self._project(self.out, self.w_out, self.rows_out, [self.branch], self._seg_out, self._out_out, None, stream)
+        self._project(self.out, self.w_out, self.rows_out, [self.branch], self._seg_out, self._out_out, self.proj_out, stream)
         native.call("qm_hc_reinject", ctypes.byref(self.ri_geom), hyper.data_ptr(), self.branch.data_ptr(),
                     self.inject.data_ptr(), hyper.data_ptr(), stream)
 
@@ -264,12 +311,16 @@ class MixDecoder:
     one per row, default every row at the layers' common position). The
     kernels read each row's position from device memory; a step replays the
     graph of the largest position's bucket, and maps each row's next page
-    first when the cache draws its pages from a pool."""
+    first when the cache draws its pages from a pool.
+
+    ``ffn``: every layer's mixture-of-experts half (reference/model.py:387-417)
+    runs behind its token-mixing half, so that a step is the whole layers'."""
 
     def __init__(self, model, cache, layers=None, dtype=torch.bfloat16, min_bucket: int = 1024, positions=None,
-                 check_every: int = 0):
+                 check_every: int = 0, ffn: bool = False):
         c = model.config
         self.model, self.cache, self.dtype = model, cache, dtype
+        self.ffn = bool(ffn)
         self.layers = list(range(len(cache.layers))) if layers is None else list(layers)
         if not self.layers:
             raise ValueError("MixDecoder needs at least one layer")
@@ -313,7 +364,7 @@ class MixDecoder:
     def _layer_steps(self, bucket: int):
         steps = self._steps.get(bucket)
         if steps is None:
-            steps = [_LayerStep(self.model, self.cache, l, bucket, self.positions, self.dtype) for l in self.layers]
+            steps = [_LayerStep(self.model, self.cache, l, bucket, self.positions, self.dtype, self.ffn) for l in self.layers]
             self._steps[bucket] = steps
         return steps
 
@@ -463,6 +514,9 @@ class MixDecoder:
             else:
                 branch = m._linear_attention(mixed, l, self.cache)
             h = m._reinject(h, branch, inject)
+            if self.ffn:
+                mixed, _, inject = m._gated_residual(h, l, "ffn", as_rows=_mix_as_rows(h.shape[0], k))
+                h = m._reinject(h, m._moe(mixed, l), inject)
         self.hyper.copy_(h[:, -1:])
         self.positions.add_(k)
         self._advance(k, host_only=True)   # the layer methods advanced the caches
@@ -473,7 +527,7 @@ class MixDecoder:
     def _layer_steps_n(self, k: int):
         steps = self._steps_n.get(k)
         if steps is None:
-            steps = [_LayerStepN(self.model, self.cache, l, k, self.positions, self.dtype) for l in self.layers]
+            steps = [_LayerStepN(self.model, self.cache, l, k, self.positions, self.dtype, self.ffn) for l in self.layers]
             self._steps_n[k] = steps
         return steps
 

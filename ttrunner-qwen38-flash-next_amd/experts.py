@@ -129,9 +129,10 @@ class MoeWeights:
         mats = (self.gate, self.up, self.down, self.s_gate, self.s_up, self.s_down)
         p = [None if t is None else t.codes.data_ptr() for t in mats]
         s = [None if t is None or t.scales is None else t.scales.data_ptr() for t in mats]
-        self._ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
-                                          native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
-        self._ptrs_ref = ctypes.byref(self._ptrs)
+        # the weights as the C ABI takes them (qm_moe_weights)
+        self.ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
+                                         native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
+        self._ptrs_ref = ctypes.byref(self.ptrs)
 
     def _take(self, mats: int, parts, what: str) -> list:
         out = []

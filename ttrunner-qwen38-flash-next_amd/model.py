@@ -10,10 +10,14 @@ return values, so an engine written against the reference can call them:
 * ``_full_attention(hidden, layer, cos, sin, cache, query_offset)``
                                                           reference/model.py:331-383
 
+and the layers' other half, ``_moe(hidden, layer)`` (reference/model.py:387-417).
+
 Weights come from ``store.get(f"blk.{layer}.{suffix}")`` as in
 reference/model.py:45-49 and are copied to the device once. The projections
 (``F.linear``) of up to 64 rows run in the library's own kernels, of more as
-PyTorch-ROCm GEMMs; everything between them -- conv ring, gates, delta rule, norms, rope, paging, indexer scoring, top-k, attention,
+PyTorch-ROCm GEMMs (with ``weight_format="mx4"`` the projections and experts are
+kept in 4-bit blocks, and every row count runs in the library's kernels);
+everything between them -- conv ring, gates, delta rule, norms, rope, paging, indexer scoring, top-k, attention,
 output gate -- runs in the HIP kernels of libqwen4mix.so. There is no other
 implementation to fall back to: a missing library or a failed call raises.
 
@@ -33,6 +37,8 @@ from torch.utils._device import DeviceContext
 from . import native
 from .cache import MixHybridCache
 from .config import MixConfig
+from .experts import MoeWeights, moe
+from .mx4 import mx4_linear, mx4_quantize
 from .rope import RopeTable
 
 
@@ -42,7 +48,13 @@ class Qwen4MixModel:
     # attention filing them itself (qm_qsa_select + qm_qsa_attend_chunk)
     fuse_chunk_select = True
 
-    def __init__(self, config, store, device=None, max_ctx: int = 8192):
+    def __init__(self, config, store, device=None, max_ctx: int = 8192, weight_format: str = "act"):
+        """``weight_format``: "act" keeps the projections and experts in the
+        activations' type, "mx4" in microscaled 4-bit blocks (quantised on first
+        use; the hyper-connections, norms, conv and routers stay as they are)."""
+        if weight_format not in ("act", "mx4"):
+            raise ValueError(f"weight_format must be 'act' or 'mx4', got {weight_format!r}")
+        self.weight_format = weight_format
         self.config = config if isinstance(config, MixConfig) else MixConfig.from_reference(config)
         self.store = store
         self.device = torch.device(device if device is not None else "cuda")
@@ -79,6 +91,7 @@ class Qwen4MixModel:
         "qsa_in": ("attn_q.weight", "attn_k.weight", "attn_v.weight", "indexer.q_proj.weight",
                    "indexer.k_proj.weight"),
         "qsa_out": ("attn_output.weight",),
+        "indexer": ("indexer.q_proj.weight", "indexer.k_proj.weight"),
     }
 
     def _wcat(self, layer: int, group: str, dtype):
@@ -99,6 +112,21 @@ class Qwen4MixModel:
             self._dev[key] = hit
         return hit
 
+    def _wcat4(self, layer: int, group: str):
+        """(Mx4Weight [N, K], rows per projection) of a projection group; a
+        row's blocks do not depend on the rows beside it."""
+        key = (layer, "mx4:" + group)
+        hit = self._dev.get(key)
+        if hit is None:
+            parts = [self.bw(layer, n).detach().to(self.device, torch.float32) for n in self.PROJ_GROUPS[group]]
+            hit = (mx4_quantize(torch.cat(parts, 0)), [int(t.shape[0]) for t in parts])
+            self._dev[key] = hit
+        return hit
+
+    def proj_weights(self, layer: int, group: str, dtype):
+        """(weights, rows per projection) of a group in the model's weight format."""
+        return self._wcat4(layer, group) if self.weight_format == "mx4" else self._wcat(layer, group, dtype)
+
     @staticmethod
     def _gemv_fits(dtype, m: int, k: int) -> bool:
         ks = (2048, 4096) if dtype == torch.bfloat16 else (1024, 2048, 4096)
@@ -115,7 +143,10 @@ class Qwen4MixModel:
     def _proj_entry(self, dtype, m: int, k: int, n_proj: int):
         """The entry point for n_proj projections of m rows over k columns (and,
         with ``_reinject`` appended, the output projection's): qm_gemv,
-        qm_gemm_rows, or None where the library's GEMM does it."""
+        qm_gemm_rows, qm_mx4_linear for 4-bit weights, or None where the
+        library's GEMM does it."""
+        if self.weight_format == "mx4":
+            return "qm_mx4_linear"
         if self._gemv_fits(dtype, m, k):
             return "qm_gemv"
         if not self._gemv_fits(dtype, 1, k):
@@ -148,7 +179,11 @@ class Qwen4MixModel:
         """The group's projections of x [B, S, K] (F.linear with each weight), as
         a list of [B, S, rows] tensors. Up to 4 rows of x: one qm_gemv launch over
         the concatenated weights; more (GEMM_ROWS_MAX): one qm_gemm_rows
-        launch; beyond: a library GEMM per projection."""
+        launch; beyond: a library GEMM per projection. 4-bit weights: one
+        qm_mx4_linear launch at any number of rows."""
+        if self.weight_format == "mx4":
+            w4, rows = self._wcat4(layer, group)
+            return mx4_linear(x, w4, sections=rows)
         dt = x.dtype
         w, rows = self._wcat(layer, group, dt)
         batch, seq, k = x.shape
@@ -230,6 +265,45 @@ class Qwen4MixModel:
         native.call("qm_hc_reinject", ctypes.byref(g), native.ptr(hyper_c), native.ptr(branch_out.contiguous()),
                     native.ptr(inject.contiguous()), native.ptr(out), native.stream_handle(hyper.device))
         return out
+
+    # -- mixture of experts (reference/model.py:387-417) -------------------------
+
+    def moe_weights(self, layer: int, dtype) -> MoeWeights:
+        """The layer's router and experts on the device, in the model's weight
+        format. A shared expert wider than the routed ones counts as several."""
+        key = (layer, "moe", dtype)
+        hit = self._dev.get(key)
+        if hit is None:
+            c = self.config
+
+            def take(suffix):
+                return self.bw(layer, suffix).detach().to(self.device, dtype if self.weight_format == "act" else torch.float32)
+
+            def lay(t):
+                return t if self.weight_format == "act" else mx4_quantize(t)
+
+            gate = lay(take("ffn_gate_exps.weight"))
+            shared = shared_router = None
+            if c.shared_expert:
+                width = int(gate.shape[1])
+                sg, su, sd = (take(f"ffn_{n}_shexp.weight") for n in ("gate", "up", "down"))
+                if sg.shape[0] % width:
+                    raise ValueError(f"layer {layer}: the shared expert is {sg.shape[0]} wide, not a multiple of the "
+                                     f"experts' {width}")
+                shared = (lay(sg.unflatten(0, (-1, width))), lay(su.unflatten(0, (-1, width))),
+                          lay(sd.unflatten(1, (-1, width)).transpose(0, 1)))
+                shared_router = self.bw(layer, "ffn_gate_inp_shexp.weight").detach().to(self.device, dtype).reshape(-1)
+            hit = MoeWeights(self.bw(layer, "ffn_gate_inp.weight").detach().to(self.device, dtype), gate,
+                             lay(take("ffn_up_exps.weight")), lay(take("ffn_down_exps.weight")),
+                             top_k=c.num_experts_per_tok, shared=shared, shared_router=shared_router,
+                             normalize=c.norm_topk_prob)
+            self._dev[key] = hit
+        return hit
+
+    def _moe(self, hidden: torch.Tensor, layer: int) -> torch.Tensor:
+        """reference/model.py:387-417: the layer's mixture of experts on hidden
+        [B, S, hidden_size]."""
+        return moe(hidden, self.moe_weights(layer, hidden.dtype))
 
     def _workspace(self, name: str, nbytes: int) -> torch.Tensor:
         buf = self._ws.get(name)
@@ -560,8 +634,11 @@ class Qwen4MixModel:
         dt = hidden.dtype
         if cache is None:
             cache = MixHybridCache(layer + 1, self.config, batch, max(kv_len, 64), self.device, dt)
-        iq = F.linear(hidden, self._dw(layer, "indexer.q_proj.weight", dt)).contiguous()
-        ik = F.linear(hidden, self._dw(layer, "indexer.k_proj.weight", dt)).contiguous()
+        if self.weight_format == "mx4":
+            iq, ik = self.project(hidden, layer, "indexer")
+        else:
+            iq = F.linear(hidden, self._dw(layer, "indexer.q_proj.weight", dt)).contiguous()
+            ik = F.linear(hidden, self._dw(layer, "indexer.k_proj.weight", dt)).contiguous()
         lc = cache[layer]
         self.qsa_core(None, None, None, iq, ik, layer, cache, query_offset, cos, sin, attend=False)
         lc.n_tokens = max(lc.n_tokens, query_offset + seq)
