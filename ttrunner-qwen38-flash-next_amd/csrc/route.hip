@@ -63,13 +63,20 @@ __device__ __forceinline__ float guard_norm(float sq, float big) {
   if (sq != sq) return INFINITY;
   return big != 0.f ? fmaxf(sq, 0x1p-126f) : sq;
 }
-__device__ __forceinline__ float oct_norm(float sq, float big) {
+// of a row of `hidden` elements, by one wave
+template <typename T> __device__ __forceinline__ float row_norm(const T* p, int hidden, int lane) {
+  constexpr int VE = 16 / sizeof(T);
+  float sq = 0.f, big = 0.f;
+  for (int u = lane; u < hidden / VE; u += 64) {
+    float v[VE];
+    unit_get(*reinterpret_cast<const uint4*>(p + (long)u * VE), v, p);
 #pragma unroll
-  for (int m = 1; m <= 4; m <<= 1) {
-    sq += __shfl_xor(sq, m, 64);
-    big = fmaxf(big, __shfl_xor(big, m, 64));
+    for (int i = 0; i < VE; ++i) {
+      sq = fmaf(v[i], v[i], sq);
+      big = fmaxf(big, fabsf(v[i]));
+    }
   }
-  return guard_norm(sq, big);
+  return guard_norm(wave_sum(sq), wave_max(big));
 }
 
 // the experts' counts of pairs, for the choice that follows
@@ -112,7 +119,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
 
 // The same by matrix cores: a workgroup per 64 router rows x 64 tokens, both kinds
 // of rows in LDS (128 k of each at a time, units exchanged as in wgemm.h), a wave
-// per 32 x 32. norms: |R[r]|^2, by the workgroups of the first tokens.
+// per 16 x 32. norms: |R[r]|^2, by the last workgroups.
 constexpr int LG_ROWS = 128;
 template <typename T> constexpr int LG_S = sizeof(T) == 2 ? 4 : 2;
 
@@ -124,6 +131,13 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
   const int e0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
+  if (blockIdx.y == gridDim.y - 1) {                         // the router rows' norms
+    for (int r = e0 + wid; r < min(e0 + 64, A.cols); r += 8) {
+      const float n = row_norm(router_row(A, r), A.hidden, lane);
+      if (lane == 0) norms[r] = n;
+    }
+    return;
+  }
   const T* src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -149,10 +163,6 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[u][i] = 0.0;
-  // thread: an eighth of router row tid / 8
-  const int n_row = threadIdx.x >> 3;
-  const bool norm = blockIdx.y == 0;
-  float sq = 0.f, big = 0.f;
   for (int j = 0; j < spans; ++j) {
     if (j + S - 2 < spans) wave_loads_barrier<(S - 2) * LOADS>();
     else wave_loads_barrier<0>();
@@ -177,22 +187,6 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
-    if (norm) {
-      for (int u = 0; u < UNITS / 8; ++u) {                  // each row from another unit on: other banks
-        const int at = (threadIdx.x & 7) * (UNITS / 8) + (u + n_row) % (UNITS / 8);
-        float v[VE];
-        unit_get(*reinterpret_cast<const uint4*>(buf + n_row * ROW_B + at * 16), v, static_cast<const T*>(nullptr));
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          sq = fmaf(v[e], v[e], sq);
-          big = fmaxf(big, fabsf(v[e]));
-        }
-      }
-    }
-  }
-  if (norm) {
-    sq = oct_norm(sq, big);
-    if ((threadIdx.x & 7) == 0 && e0 + n_row < A.cols) norms[e0 + n_row] = sq;
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -214,34 +208,49 @@ struct TopArgs {
   const float* norms;  // null: the logits are sums in double already
 };
 
-// The logit of expert e in double, by 32 lanes
+// The logits of four experts in double, by the wave: lane c < 4 gets expert c's. One
+// round trip for all of them; the lanes' partial sums meet in the order of their
+// numbers' bits, whichever four are asked for.
+constexpr int EXACT = 4;
 template <typename T>
-__device__ __forceinline__ double exact_logit(const QmLogits<T>& A, int t, int e, int l32) {
-  constexpr int VE = 16 / sizeof(T);
-  const T* w = A.router + (long)e * A.hidden;
-  const T* x = A.x + (long)t * A.ldx;
-  constexpr int B = 8;                     // loads in flight: the sum is a chain of latencies otherwise
+__device__ __forceinline__ double exact_logits(const QmLogits<T>& A, int t, const int (&e)[EXACT], int lane) {
+  constexpr int VE = 16 / sizeof(T), B = 4;                  // units of a lane in flight
   const int units = A.hidden / VE;
-  double s = 0.0;
-  for (int u0 = l32; u0 < units; u0 += 32 * B) {
-    uint4 wu[B], xu[B];
+  const T* x = A.x + (long)t * A.ldx;
+  double s[EXACT];
+#pragma unroll
+  for (int c = 0; c < EXACT; ++c) s[c] = 0.0;
+  for (int u0 = lane; u0 < units; u0 += 64 * B) {
+    uint4 xu[B], wu[EXACT][B];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      const long at = (long)min(u0 + 32 * b, units - 1) * VE;
-      wu[b] = *reinterpret_cast<const uint4*>(w + at);
+      const long at = (long)min(u0 + 64 * b, units - 1) * VE;
       xu[b] = *reinterpret_cast<const uint4*>(x + at);
+#pragma unroll
+      for (int c = 0; c < EXACT; ++c) wu[c][b] = *reinterpret_cast<const uint4*>(A.router + (long)e[c] * A.hidden + at);
     }
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      if (u0 + 32 * b >= units) break;
-      float wv[VE], xv[VE];
-      unit_get(wu[b], wv, w);
-      unit_get(xu[b], xv, w);
+      if (u0 + 64 * b >= units) break;
+      float xv[VE];
+      unit_get(xu[b], xv, x);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) s = exact_fma(wv[i], xv[i], s, w);
+      for (int c = 0; c < EXACT; ++c) {
+        float wv[VE];
+        unit_get(wu[c][b], wv, x);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) s[c] = exact_fma(wv[i], xv[i], s[c], x);
+      }
     }
   }
-  return lanes_sum_f64<32>(s);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1)
+#pragma unroll
+    for (int c = 0; c < EXACT; ++c) s[c] += __shfl_xor(s[c], m, 64);
+  double mine = s[0];
+#pragma unroll
+  for (int c = 1; c < EXACT; ++c) mine = lane == c ? s[c] : mine;
+  return mine;
 }
 
 // The workgroup that finishes last makes the table of row tiles from the counts,
@@ -338,25 +347,10 @@ __global__ __launch_bounds__(LS_NT) void moe_lists_kernel(const int* ids, int ro
 template <typename T, int PER>
 __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P, int t, int lane) {
   double* l = A.logits + (long)t * A.cols;
-  WaveTop<PER> top;
-  float sq = 0.f, big = 0.f;               // of the token's row
-  if (P.norms) {
-    constexpr int VE = 16 / sizeof(T);
-    for (int u = lane; u < A.hidden / VE; u += 64) {
-      float v[VE];
-      unit_get(*reinterpret_cast<const uint4*>(A.x + (long)t * A.ldx + (long)u * VE), v, A.x);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        sq = fmaf(v[i], v[i], sq);
-        big = fmaxf(big, fabsf(v[i]));
-      }
-    }
-  }
-  top.load(l, A.experts, lane);
-  // 2 B: logits further apart are in the right order
-  double close = -1.0;
+  double off = 0.0;                        // the logits' own error
   bool all = false;                        // every logit has to be summed again
   if (P.norms) {
+    const float xn = row_norm(A.x + (long)t * A.ldx, A.hidden, lane);
     float wn = 0.f;
     bool bad = false;
 #pragma unroll
@@ -367,81 +361,28 @@ __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P,
       wn = fmaxf(wn, v);
       bad |= !(v < INFINITY) || !(fabs(l[e]) < (double)INFINITY);
     }
-    const float xn = guard_norm(wave_sum(sq), wave_max(big));
     wn = wave_max(wn);
     // squares below float's range hide a norm
     all = __builtin_amdgcn_ballot_w64(bad) != 0ull || !(xn < INFINITY) || (xn != 0.f && (xn < 0x1p-80f || wn < 0x1p-80f));
     // (a row of zeros has logits of zero; the norms' own rounding is far below 2^-10)
-    if (all) close = 0.0;
-    else if (xn != 0.f) close = 2.0 * (129.0 * 0x1p-23 * (1.0 + 0x1p-10) * sqrt((double)xn * (double)wn) + A.hidden * 0x1p-126);
+    if (xn != 0.f) off = 129.0 * 0x1p-23 * (1.0 + 0x1p-10) * sqrt((double)xn * (double)wn) + A.hidden * 0x1p-126;
   }
-  int n = 0, id = 0x7fffffff;
-  long long key = KEY_GONE;                // lane j: the j-th largest
-  if (!all) {
-    double bar = 0.0;                      // the top_k-th logit - 2 B
-    const int most = close < 0.0 ? P.top_k : A.experts;
-    for (; n < most; ++n) {
-      long long best;
-      const int at = top.take(lane, best);
-      const double v = key_logit(best);
-      if (n == P.top_k - 1) bar = v - close;
-      if (n >= P.top_k && v < bar) break;
-      if (n == 64) { all = true; break; }  // more candidates than lanes
-      if (lane == n) { key = best; id = at; }
-    }
-  }
-  if (close >= 0.0) {
-    if (!all) {
-      // neighbours closer than 2 B: both in double
-      const double v = key_logit(key), above = __shfl_up(v, 1, 64), below = __shfl_down(v, 1, 64);
-      const bool again = lane < n && ((lane > 0 && above - v <= close) || (lane + 1 < n && v - below <= close));
-      const unsigned long long close_ones = __builtin_amdgcn_ballot_w64(again);
-      unsigned long long m = close_ones;
-      while (m) {
-        // two at a time; the other half repeats the first where there is one
-        const int first = __ffsll(m) - 1;
-        m &= m - 1;
-        const int second = m ? __ffsll(m) - 1 : first;
-        m &= m - 1;
-        const int e = lane < 32 ? __builtin_amdgcn_readlane(id, first) : __builtin_amdgcn_readlane(id, second);
-        const double s = exact_logit(A, t, e, lane & 31);
-        const long long k = logit_key(s);
-        const long long k0 = lane_key(k, 0), k1 = lane_key(k, 32);
-        if (lane == first) key = k0;
-        if (lane == second) key = k1;
-      }
-      // their order again
-      int rank = 0;
-      for (int i = 0; close_ones && i < n; ++i) {
-        const long long ok = lane_key(key, i);
-        const int oi = __builtin_amdgcn_readlane(id, i);
-        rank += ok > key || (ok == key && oi < id);
-      }
-      long long sorted_key = key;
-      int sorted_id = id;
-      for (int i = 0; close_ones && i < n; ++i) {
-        const int at = __builtin_amdgcn_readlane(rank, i);
-        const long long ok = lane_key(key, i);
-        const int oi = __builtin_amdgcn_readlane(id, i);
-        if (lane == at) { sorted_key = ok; sorted_id = oi; }
-      }
-      key = sorted_key;
-      id = sorted_id;
-    } else {
-      for (int e0 = 0; e0 < A.experts; e0 += 2) {
-        const int e = min(e0 + (lane >> 5), A.experts - 1);
-        const double s = exact_logit(A, t, e, lane & 31);
-        if ((lane & 31) == 0 && e0 + (lane >> 5) < A.experts) l[e] = s;
+  long long key;                           // lane j: the j-th largest
+  int id;
+  if (!all)
+    all = !wave_topk<PER>(l, A.experts, P.top_k, off, lane, key, id,
+                          [&](const int (&e)[4]) { return exact_logits(A, t, e, lane); });
+  if (all) {
+    if (P.norms) {
+      for (int e0 = 0; e0 < A.experts; e0 += EXACT) {
+        const int last = A.experts - 1, e[EXACT] = {e0, min(e0 + 1, last), min(e0 + 2, last), min(e0 + 3, last)};
+        const double s = exact_logits(A, t, e, lane);
+        if (lane < EXACT && e0 + lane < A.experts) l[e0 + lane] = s;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       wait_all_memory();
-      top.load(l, A.experts, lane);
-      for (n = 0; n < P.top_k; ++n) {
-        long long best;
-        const int at = top.take(lane, best);
-        if (lane == n) { key = best; id = at; }
-      }
     }
+    wave_topk_exact(l, A.experts, P.top_k, lane, key, id);
   }
   const double v0 = key_logit(lane_key(key, 0));
   const float mine = lane < P.top_k ? expf((float)(key_logit(key) - v0)) : 0.f;
@@ -507,7 +448,7 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
     const size_t lds = (size_t)LG_S<T> * LG_ROWS * WT_K * sizeof(T);
     rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds);
     if (rc) return rc;
-    hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64, (A.rows + 63) / 64), dim3(512), lds, stream, A, norms);
+    hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64, (A.rows + 63) / 64 + 1), dim3(512), lds, stream, A, norms);
     QM_CHECK_LAUNCH();
   }
   if (rc) return rc;

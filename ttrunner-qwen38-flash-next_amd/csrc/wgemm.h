@@ -6,7 +6,8 @@
 // one barrier a span. Weights arrive in operand order; an activation row's 16-byte
 // units are exchanged by an exclusive or with its number, so that the 16 rows of
 // an operand read distinct banks. 4-bit weights become bf16 in the registers of
-// the waves that multiply them.
+// the waves that multiply them. STREAM: the weights are read once or twice (few row
+// tiles) and are not kept in the L2 before the activations.
 #pragma once
 
 #include "wtile.h"
@@ -18,7 +19,7 @@ __device__ __forceinline__ int xcd_run(int bid, int n) {
   return x * q + min(x, r) + bid / 8;
 }
 
-template <typename WF, typename T, int TN, int TM, int WN, int WM, int S>
+template <typename WF, typename T, int TN, int TM, int WN, int WM, int S, bool STREAM = false>
 struct SpanGemm {
   using F = Fmt<WF, T>;
   static constexpr int NW = WN * WM;
@@ -68,7 +69,12 @@ struct SpanGemm {
       if (row < rows) lds_load16(p, buf + at);                // (rows past the last multiply what lies there, unread)
     }
 #pragma unroll
-    for (int i = 0; i < WL; ++i) lds_load16(src.w[i] + (long)j * F::SPAN_B, buf + X_B + (wid * WL + i) * 1024);
+    for (int i = 0; i < WL; ++i) {
+      const char* p = src.w[i] + (long)j * F::SPAN_B;
+      char* to = buf + X_B + (wid * WL + i) * 1024;
+      if constexpr (STREAM) lds_load16_stream(p, to);
+      else lds_load16(p, to);
+    }
     if constexpr (F::SCALED) lds_load4(src.s + (long)j * 64, buf + X_B + W_B + wid * 256);
   }
   __device__ __forceinline__ static void run(f32x4_t (&acc)[TN][TM], char* lds, const Src& src, int k, int rows) {

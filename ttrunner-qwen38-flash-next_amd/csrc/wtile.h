@@ -252,6 +252,11 @@ __device__ __forceinline__ void lds_load16(const void* p, char* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
+// (the non-temporal form: not kept in the L2 before what is read more often)
+__device__ __forceinline__ void lds_load16_stream(const void* p, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 2);
+}
 __device__ __forceinline__ void lds_load4(const void* p, char* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                    (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
