@@ -57,7 +57,7 @@ def _project(entry, act, rows, x, w, sizes, outs, seg_rows, seg_out, stream):
     by library GEMMs where that is None."""
     if entry == "qm_mx4_linear":
         n, k = w.shape
-        native.call(entry, act, rows, n, k, w.codes.data_ptr(), w.scales.data_ptr(), x.data_ptr(), k, len(sizes),
+        native.call(entry, act, rows, n, k, w.codes_ptr, w.scales_ptr, x.data_ptr(), k, len(sizes),
                     seg_rows, seg_out, stream)
         return
     if entry:

@@ -80,10 +80,10 @@ class _Tiles:
         self.shape = w.shape
         wc = dense(w)
         tiles = -(-n // 16) * -(-k // 128)
-        self.codes = torch.empty(mats * tiles * 2048, dtype=w.dtype, device=w.device)
-        self.scales = None
+        self.data = torch.empty(mats * tiles * 2048, dtype=w.dtype, device=w.device)
+        self.codes_ptr, self.scales_ptr = self.data.data_ptr(), None
         with on_device(w.device):
-            native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), native.ptr(self.codes),
+            native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), self.codes_ptr,
                         stream_of(w.device))
 
 
@@ -127,8 +127,8 @@ class MoeWeights:
         elif shared_router is not None:
             raise ValueError("shared_router without shared experts")
         mats = (self.gate, self.up, self.down, self.s_gate, self.s_up, self.s_down)
-        p = [None if t is None else t.codes.data_ptr() for t in mats]
-        s = [None if t is None or t.scales is None else t.scales.data_ptr() for t in mats]
+        p = [None if t is None else t.codes_ptr for t in mats]
+        s = [None if t is None else t.scales_ptr for t in mats]
         # the weights as the C ABI takes them (qm_moe_weights)
         self.ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
                                          native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])

@@ -77,15 +77,28 @@ def activation_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 class Mx4Weight:
     """A weight [..., n, k] in 4-bit blocks along k, laid out for the kernels.
 
-    ``codes`` and ``scales`` are the device tiles; ``plain()`` gives them in a
-    checkpoint's order, ``dequantize()`` the values they stand for."""
+    ``data`` holds the device tiles, ``codes`` and ``scales`` are views of it;
+    ``plain()`` gives them in a checkpoint's order, ``dequantize()`` the values they
+    stand for."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
-        self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
+    def __init__(self, data: torch.Tensor, shape):
+        self.data, self.shape = data, torch.Size(shape)
+        # the codes are 16 of 17 bytes, the scales behind them
+        self.code_bytes = data.numel() // 17 * 16
+        self.codes_ptr = data.data_ptr()
+        self.scales_ptr = self.codes_ptr + self.code_bytes
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[:self.code_bytes]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.code_bytes:]
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     @property
     def mats(self) -> int:
@@ -103,11 +116,8 @@ class Mx4Weight:
     def _empty(cls, shape, device) -> "Mx4Weight":
         shape = torch.Size(shape)
         cls._check_shape(shape)
-        nbytes = native.load().qm_mx4_code_bytes(shape[:-2].numel(), shape[-2], shape[-1])
-        if not nbytes:
-            raise ValueError(f"unsupported size of a 4-bit weight: {tuple(shape)}")
-        return cls(torch.empty(nbytes, dtype=torch.uint8, device=device),
-                   torch.empty(nbytes // 16, dtype=torch.uint8, device=device), shape)
+        tiles = shape[:-2].numel() * -(-shape[-2] // TILE_ROWS) * -(-shape[-1] // TILE_K)
+        return cls(torch.empty(tiles * (TILE_ROWS * TILE_K // 32 * 17), dtype=torch.uint8, device=device), shape)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mx4Weight":
@@ -124,7 +134,7 @@ class Mx4Weight:
         w = cls._empty(shape, codes.device)
         pc, ps = dense(codes), scales.contiguous()
         with on_device(codes.device):
-            native.call("qm_mx4_layout", 1, w.mats, shape[-2], shape[-1], native.ptr(w.codes), native.ptr(w.scales),
+            native.call("qm_mx4_layout", 1, w.mats, shape[-2], shape[-1], w.codes_ptr, w.scales_ptr,
                         native.ptr(pc), native.ptr(ps), stream_of(codes.device))
         return w
 
@@ -134,18 +144,19 @@ class Mx4Weight:
         codes = torch.empty(*lead, n, k // 2, dtype=torch.uint8, device=self.device)
         scales = torch.empty(*lead, n, k // BLOCK, dtype=torch.uint8, device=self.device)
         with on_device(self.device):
-            native.call("qm_mx4_layout", 0, self.mats, n, k, native.ptr(self.codes), native.ptr(self.scales),
+            native.call("qm_mx4_layout", 0, self.mats, n, k, self.codes_ptr, self.scales_ptr,
                         native.ptr(codes), native.ptr(scales), stream_of(self.device))
         return codes, scales
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values, [..., n, k]: exact in float32 and in bfloat16 (a value past
         their range is infinite)."""
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with on_device(self.device):
-            native.call("qm_mx4_dequantize", native.act_code(dtype), self.mats, self.shape[-2], self.shape[-1],
-                        native.ptr(self.codes), native.ptr(self.scales), native.ptr(out),
-                        stream_of(self.device))
+        shape, device = self.shape, self.data.device
+        act = native.act_code(dtype)
+        out = torch.empty(shape, dtype=dtype, device=device)
+        with on_device(device):
+            native.check("qm_mx4_dequantize", native.load().qm_mx4_dequantize(
+                act, self.mats, shape[-2], shape[-1], self.codes_ptr, self.scales_ptr, out.data_ptr(), stream_of(device)))
         return out
 
 
@@ -154,12 +165,13 @@ def mx4_quantize(w: torch.Tensor) -> Mx4Weight:
     4-bit blocks: the scale 2^max(floor(log2 max|w|) - 2, -127), the elements to
     the nearest value, ties to the even code, magnitudes above 6 scales to 6. A
     block that holds a NaN or an infinity becomes NaN."""
-    check_input(w, "w")
-    out = Mx4Weight._empty(w.shape, w.device)
+    act = check_input(w, "w")
+    shape, device = w.shape, w.device
+    out = Mx4Weight._empty(shape, device)
     wc = dense(w)
-    with on_device(w.device):
-        native.call("qm_mx4_quantize", native.act_code(w.dtype), out.mats, w.shape[-2], w.shape[-1], native.ptr(wc),
-                    native.ptr(out.codes), native.ptr(out.scales), stream_of(w.device))
+    with on_device(device):
+        native.check("qm_mx4_quantize", native.load().qm_mx4_quantize(
+            act, out.mats, shape[-2], shape[-1], wc.data_ptr(), out.codes_ptr, out.scales_ptr, stream_of(device)))
     return out
 
 
@@ -193,6 +205,6 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Weight, sections=None):
         seg_out = (ctypes.c_void_p * len(rows))(*[o.data_ptr() for o in outs])
         with on_device(device):
             native.check("qm_mx4_linear", native.load().qm_mx4_linear(
-                act, m, n, k, weight.codes.data_ptr(), weight.scales.data_ptr(), xr.data_ptr(), ldx, len(rows), seg_rows,
+                act, m, n, k, weight.codes_ptr, weight.scales_ptr, xr.data_ptr(), ldx, len(rows), seg_rows,
                 seg_out, stream_of(device)))
     return outs[0] if sections is None else outs
