@@ -80,6 +80,93 @@ def test_route_does_not_depend_on_the_rows_beside(gpu):
         assert ((part_w.double() / w[lo:hi].double() - 1).abs().max().item()) < W_TOL
 
 
+# Many rows: the logits come from the matrix cores and only close ones are summed
+# again. A logit is then off by at most B = (129 2^-23) |x| |R[e]|; a weight, the
+# exponential of a difference over a sum of such, by 4 B relative. Over all weights
+# (|x| = h^1/2, |R[e]| = 1): each of a block's 128 additions is off by less than a
+# step of a partial sum whose mean is 0.67 (128 / h)^1/2 at its end, all in one
+# direction at worst, h / 128 blocks: 4.1e-5 a logit at h = 2080, 2^-14 for the
+# difference of two.
+MANY = [(500, 130, 8, 2080), (130, 1024, 32, 1056), (1700, 60, 4, 1024), (3300, 16, 2, 2048), (1001, 257, 1, 416)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,e,k,h", MANY)
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_many_rows(gpu, dtype, t, e, k, h, normalize):
+    assert t * e * h > 1e8
+    x, r = normal(t + e, t, h, dtype=dtype), normal(h, e, h, dtype=dtype, scale=h ** -0.5)
+    ids, w = gpu.moe_route(x, r, k, normalize)
+    want_ids, want_w = fo.route(x, r, k, normalize)
+    assert torch.equal(ids, want_ids)
+    rel = (w.double() - want_w).abs() / want_w
+    lim = W_TOL + 4 * 129 * 2.0 ** -23 * x.double().norm(dim=-1) * r.double().norm(dim=-1).max()
+    assert record("bound", (rel / lim[:, None]).max().item(), 1.0) <= 1.0
+    rms = rel.square().mean().sqrt().item()
+    assert record("rms", rms, 2.0 ** -14) < 2.0 ** -14
+    for lo, hi in ((0, 1), (63, 66), (t - 20, t)):                  # as the same rows alone
+        assert torch.equal(gpu.moe_route(x[lo:hi], r, k, normalize)[0], ids[lo:hi])
+    base = torch.zeros(t, h + 64, dtype=dtype, device=DEV)
+    base[:, 32:32 + h] = x                                          # rows apart
+    ids2, w2 = gpu.moe_route(base[:, 32:32 + h], r, k, normalize)
+    assert torch.equal(ids2, ids) and torch.equal(w2, w)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("copies", [3, 40, 150])
+def test_route_many_rows_close_logits(gpu, dtype, copies):
+    """Router rows a last bit apart (the order takes sums in double) and equal ones."""
+    t, e, h, k = 600, 160, 1184, 12
+    x = normal(1, t, h, dtype=dtype)
+    r = normal(2, e, h, dtype=dtype, scale=h ** -0.5)
+    near = torch.randperm(e, generator=torch.Generator().manual_seed(3))[:copies].tolist()
+    r[near] = r[near[0]].clone()
+    for i, n in enumerate(near):
+        if i % 3:                                                   # every third stays equal
+            r[n, i] += r[n, i] * torch.finfo(dtype).eps
+    x += 3 * r[near[0]]
+    ids, w = gpu.moe_route(x, r, k)
+    assert torch.equal(ids, fo.route(x, r, k)[0])
+    assert torch.equal(gpu.moe_route(x[77:80], r, k)[0], ids[77:80])
+    assert bool((w[:, :-1] >= w[:, 1:]).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_route_many_rows_ties_magnitudes_and_bad_values(gpu, dtype):
+    t, e, h, k = 700, 96, 1632, 6
+    r = normal(2, e, h, dtype=dtype, scale=h ** -0.5)
+    x = normal(1, t, h, dtype=dtype)
+    x *= torch.logspace(-38, 17, t, device=DEV).to(dtype)[:, None]
+    x[5] = 0
+    x[6] = 0
+    x[6, 9] = torch.finfo(dtype).tiny
+    ids, w = gpu.moe_route(x, r, k)
+    want = fo.route(x, r, k)[0]
+    assert torch.equal(ids, want) and ids[5].tolist() == list(range(k))
+    assert bool((w.sum(-1) - 1).abs().max() < 2.0 ** -20) and bool((w[5] == w[5, 0]).all())
+    small = normal(4, e, h, dtype=dtype, scale=1e-30)               # products below float's range
+    tiny_ids = gpu.moe_route(x[:400], small, k)[0] if 400 * e * h > 1e8 else gpu.moe_route(x, small, k)[0]
+    assert torch.equal(tiny_ids, fo.route(x, small, k)[0][:tiny_ids.shape[0]])
+    zero = torch.zeros_like(x)
+    ids0, w0 = gpu.moe_route(zero, r, k)
+    assert ids0.tolist() == [list(range(k))] * t and torch.equal(w0, torch.full_like(w0, w0[0, 0].item()))
+    x = normal(1, t, h, dtype=dtype)
+    clean, cw = gpu.moe_route(x, r, k)
+    bad = x.clone()
+    bad[0, 3], bad[64, h - 1], bad[t - 1, 0], bad[300] = float("nan"), float("inf"), float("-inf"), float("nan")
+    ids, w = gpu.moe_route(bad, r, k)
+    hit = [0, 64, 300, t - 1]
+    for i in hit:
+        alone_ids, alone_w = gpu.moe_route(bad[i:i + 1], r, k)
+        assert torch.equal(ids[i:i + 1], alone_ids) and bool(w[i].isnan().all()) and bool(alone_w.isnan().all())
+    keep = [i for i in range(t) if i not in hit]
+    assert torch.equal(ids[keep], clean[keep]) and torch.equal(w[keep], cw[keep])
+    r2 = r.clone()
+    r2[70, 1] = float("nan")
+    ids, w = gpu.moe_route(x, r2, k)
+    assert bool((ids[:, 0] == 70).all()) and bool(w.isnan().all())
+
+
 def layer(qm, seed, e, h, i, shared, top_k, fmt, dtype, gated=True, normalize=True, bias=None):
     """(MoeWeights, the oracle's arguments)."""
     router = normal(seed, e, h, dtype=dtype, scale=h ** -0.5)
@@ -125,6 +212,40 @@ def test_moe_matches_f64(gpu, dtype, fmt, t, e, k, h, i, shared):
     w, args = layer(gpu, t + e, e, h, i, shared, k, fmt, dtype, gated=t % 2 == 1, normalize=t % 3 != 0)
     x = normal(t, t, h, dtype=dtype)
     check(gpu.moe(x, w), x, args)
+
+
+# the borders between the kernels: 16 and 17 tokens; row tiles of 64 and 128; experts'
+# lists by the choosing waves and apart, over one round of choices and several;
+# weights read once; logits by matrix cores; the largest top_k, experts and shared
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t,e,k,h,i,shared", [(16, 24, 4, 288, 160, 1), (17, 24, 4, 288, 160, 1), (300, 8, 2, 160, 96, 1),
+                                              (1100, 4, 2, 160, 96, 1), (3000, 32, 6, 64, 32, 0), (290, 24, 2, 96, 64, 0),
+                                              (280, 24, 2, 96, 64, 1), (1700, 60, 4, 1056, 32, 1), (16, 1024, 32, 32, 32, 1),
+                                              (40, 1024, 32, 32, 32, 0), (3, 32, 32, 64, 32, 32), (20, 32, 32, 64, 32, 32),
+                                              (16, 1, 1, 96, 32, 0), (90, 1, 1, 96, 32, 0)])
+def test_moe_borders(gpu, fmt, t, e, k, h, i, shared):
+    print(f"moe {fmt} t={t} e={e} k={k} h={h} i={i} shared={shared}", flush=True)
+    w, args = layer(gpu, t + e, e, h, i, shared, k, fmt, BF16, normalize=t % 2 == 0)
+    x = normal(t, t, h, dtype=BF16)
+    check(gpu.moe(x, w), x, args)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t", [1, 9, 60, 400])
+def test_calls_on_two_streams_at_once(gpu, fmt, t):
+    w, args = layer(gpu, 21, 16, 256, 128, 1, 4, fmt, BF16)
+    xs = [normal(60 + i, t, 256, dtype=BF16) for i in range(2)]
+    want = [gpu.moe(x, w) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(gpu.moe(xs[i], w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, y) for gs, y in zip(got, want) for g in gs)
 
 
 @pytest.mark.parametrize("fmt", ["plain", "mx4"])

@@ -123,6 +123,34 @@ def test_linear_keeps_bad_values_to_their_rows(gpu, dtype, m):
     assert bool(bad[:, 11].isnan().all()) and bool(bad[:, :11].isfinite().all()) and bool(bad[:, 12:].isfinite().all())
 
 
+# One size for each tiling that many rows can take (the workgroups that a tile
+# leaves decide), at the smallest k that still ends inside a tile of 128.
+TILINGS = [(40, 300), (100, 4090), (300, 4090), (600, 4090), (1030, 4090), (2000, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n", TILINGS)
+@pytest.mark.parametrize("k", [160, 416])
+def test_linear_tilings(gpu, dtype, m, n, k):
+    q = gpu.mx4_quantize(normal(n, n, k, dtype=dtype, scale=k ** -0.5))
+    base = normal(m + k, m, k + 64, dtype=dtype)
+    x = base[:, 32:32 + k]                                          # rows apart
+    want, bound = fo.linear(x, q.dequantize(F32))
+    got = gpu.mx4_linear(x, q)
+    assert record("bound", fo.within(got, want, bound, dtype), 1.0) <= 1.0
+    lim = 2 * fo.half(dtype) if dtype == BF16 else 2 ** -19
+    assert record("norm", ((got.double() - want).norm() / want.norm()).item(), lim) < lim
+    parts = gpu.mx4_linear(x, q, sections=[17, n - 19, 2])
+    assert torch.equal(torch.cat(parts, -1), got)
+    bad = x.clone()
+    bad[m // 2, k - 1], bad[m - 1, 0] = float("nan"), float("inf")
+    spoilt = gpu.mx4_linear(bad, q)
+    assert bool(spoilt[m // 2].isnan().all()) and not bool(spoilt[m - 1].isfinite().all())
+    keep = torch.arange(m, device=DEV)
+    keep = keep[(keep != m // 2) & (keep != m - 1)]
+    assert torch.equal(spoilt[keep], got[keep])
+
+
 def test_linear_float_activations_keep_their_bits(gpu):
     """A float activation enters as three bf16 parts: against a weight of ones in
     one block, sums of few terms are exact."""
@@ -153,6 +181,23 @@ def test_linear_on_a_side_stream_and_in_a_graph(gpu):
         gpu.mx4_linear(x, q)                                        # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("m", [3, 40, 700])
+def test_linear_calls_on_two_streams_at_once(gpu, m):
+    q = gpu.mx4_quantize(normal(9, 2000, 512, dtype=BF16))
+    xs = [normal(40 + i, m, 512, dtype=BF16) for i in range(2)]
+    want = [gpu.mx4_linear(x, q) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(gpu.mx4_linear(xs[i], q))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
 
 
 def test_refusals(gpu):

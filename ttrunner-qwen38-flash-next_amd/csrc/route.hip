@@ -41,9 +41,8 @@ __device__ __forceinline__ void unit_get(const uint4& c, float (&v)[4], const fl
   v[0] = __uint_as_float(c.x); v[1] = __uint_as_float(c.y); v[2] = __uint_as_float(c.z); v[3] = __uint_as_float(c.w);
 }
 
-// s + w x in double: a product of bf16 is exact in float
-__device__ __forceinline__ double exact_fma(float w, float x, double s, const bf16_t*) { return s + (double)(w * x); }
-__device__ __forceinline__ double exact_fma(float w, float x, double s, const float*) { return fma((double)w, (double)x, s); }
+// s + w x in double (a product of two bf16 fits a float's bits, but not its range)
+__device__ __forceinline__ double exact_fma(float w, float x, double s) { return fma((double)w, (double)x, s); }
 
 template <int LANES> __device__ __forceinline__ double lanes_sum_f64(double v) {
 #pragma unroll
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
       float xv[VE];
       unit_get(*reinterpret_cast<const uint4*>(A.x + (long)(t0 + i) * A.ldx + (long)u * VE), xv, w);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[i] = exact_fma(wv[e], xv[e], acc[i], w);
+      for (int e = 0; e < VE; ++e) acc[i] = exact_fma(wv[e], xv[e], acc[i]);
     }
   }
 #pragma unroll
@@ -239,7 +238,7 @@ __device__ __forceinline__ double exact_logits(const QmLogits<T>& A, int t, cons
         float wv[VE];
         unit_get(wu[c][b], wv, x);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) s[c] = exact_fma(wv[i], xv[i], s[c], x);
+        for (int i = 0; i < VE; ++i) s[c] = exact_fma(wv[i], xv[i], s[c]);
       }
     }
   }
