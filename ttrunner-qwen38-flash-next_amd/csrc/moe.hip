@@ -81,7 +81,7 @@ template <int PER>
 __device__ __forceinline__ int wave_choose(const double* l, int experts, int top_k, int normalize, int lane, float& weight) {
   long long key;
   int id;
-  if (!wave_topk<PER>(l, experts, top_k, 0.0, lane, key, id, [](const int (&)[4]) { return 0.0; }))
+  if (!wave_topk<PER>(l, experts, top_k, 0.0, lane, key, id, [](const int (&)[RT_EXACT]) { return 0.0; }))
     wave_topk_exact(l, experts, top_k, lane, key, id);
   const double v0 = key_logit(lane_key(key, 0));
   const float mine = lane < top_k ? expf((float)(key_logit(key) - v0)) : 0.f;
@@ -467,7 +467,7 @@ MoeLayout moe_layout(const qm_moe_geom& g) {
     l.bm = rows_per_tile(g);
     // every expert's last tile may be part-filled
     l.max_tiles = (long)(choices / l.bm + hot + g.shared * ((t + l.bm - 1) / l.bm));
-    l.norms = take(qm_route_norms(g.experts));
+    l.norms = take(qm_route_norms(g.rows, g.experts));
     l.ids = take(choices * sizeof(int));
     l.pair_w = take(pairs * sizeof(float));
     l.counts = take((g.experts + 1) * sizeof(int));           // and the number of finished workgroups

@@ -21,7 +21,7 @@ struct QmLogits {
 };
 
 // float words of the scratch that qm_route needs beside the logits, in bytes
-size_t qm_route_norms(int experts);
+size_t qm_route_norms(int rows, int experts);
 
 // The logits of a few rows, summed in double (one launch).
 template <typename T> int qm_route_logits(const QmLogits<T>& A, hipStream_t stream);

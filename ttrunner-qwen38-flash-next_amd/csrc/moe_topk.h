@@ -6,6 +6,7 @@
 
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_TOPK = 32;
+constexpr int RT_EXACT = 2;
 
 // A logit as an integer of the same order: NaN above everything, +0 and -0 equal.
 __device__ __forceinline__ long long logit_key(double v) {
@@ -83,8 +84,8 @@ struct WaveTop {
 
 // The top_k largest logits of a token in the doubles' order, one per lane (key, id
 // of lane j < top_k), by one wave. The logits in l are off by up to `off` each (0:
-// they are the doubles); exact(e[4]) gives the sums in double of four experts to
-// lanes 0 to 3. False, with nothing chosen, when more of them come close than a
+// they are the doubles); exact(e[2]) gives the sums in double of two experts to
+// lanes 0 and 1. False, with nothing chosen, when more of them come close than a
 // wave holds.
 template <int PER, typename Exact>
 __device__ __forceinline__ bool wave_topk(const double* l, int experts, int top_k, double off, int lane, long long& key,
@@ -120,17 +121,17 @@ __device__ __forceinline__ bool wave_topk(const double* l, int experts, int top_
   unsigned long long m = __builtin_amdgcn_ballot_w64(again);
   if (m == 0ull) return true;
   while (off > 0.0 && m) {
-    // four at a time; the last of them again where there are fewer
-    int at[4], e[4];
+    // the last of them again where there is no other
+    int at[RT_EXACT], e[RT_EXACT];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < RT_EXACT; ++c) {
       at[c] = m ? __ffsll(m) - 1 : at[c - 1 < 0 ? 0 : c - 1];
       m &= m - 1;
       e[c] = __builtin_amdgcn_readlane(id, at[c]);
     }
     const long long k = logit_key(exact(e));
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < RT_EXACT; ++c) {
       const long long kc = lane_key(k, c);
       if (lane == at[c]) key = kc;
     }
@@ -142,16 +143,10 @@ __device__ __forceinline__ bool wave_topk(const double* l, int experts, int top_
     const int oi = __builtin_amdgcn_readlane(id, i);
     rank += ok > key || (ok == key && oi < id);
   }
-  long long sorted_key = key;
-  int sorted_id = id;
-  for (int i = 0; i < n; ++i) {
-    const int at = __builtin_amdgcn_readlane(rank, i);
-    const long long ok = lane_key(key, i);
-    const int oi = __builtin_amdgcn_readlane(id, i);
-    if (lane == at) { sorted_key = ok; sorted_id = oi; }
-  }
-  key = sorted_key;
-  id = sorted_id;
+  if (lane >= n) rank = lane;              // a permutation of the lanes
+  const int lo = __builtin_amdgcn_ds_permute(4 * rank, (int)key), hi = __builtin_amdgcn_ds_permute(4 * rank, (int)(key >> 32));
+  key = (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+  id = __builtin_amdgcn_ds_permute(4 * rank, id);
   return true;
 }
 

@@ -16,7 +16,7 @@
 // summed again in double (about one token in ten of normal rows has such a pair).
 #include "moe_internal.h"
 #include "moe_topk.h"
-#include "wtile.h"
+#include "wgemm.h"
 
 namespace {
 
@@ -53,29 +53,6 @@ template <int LANES> __device__ __forceinline__ double lanes_sum_f64(double v) {
 template <typename T>
 __device__ __forceinline__ const T* router_row(const QmLogits<T>& A, int r) {
   return r < A.experts ? A.router + (long)r * A.hidden : A.shared_router;
-}
-
-// The square of a row's norm from partial sums of squares and largest magnitudes
-// over groups of lanes: zero only of a row of zeros, infinite where a NaN or an
-// infinity is in it.
-__device__ __forceinline__ float guard_norm(float sq, float big) {
-  if (sq != sq) return INFINITY;
-  return big != 0.f ? fmaxf(sq, 0x1p-126f) : sq;
-}
-// of a row of `hidden` elements, by one wave
-template <typename T> __device__ __forceinline__ float row_norm(const T* p, int hidden, int lane) {
-  constexpr int VE = 16 / sizeof(T);
-  float sq = 0.f, big = 0.f;
-  for (int u = lane; u < hidden / VE; u += 64) {
-    float v[VE];
-    unit_get(*reinterpret_cast<const uint4*>(p + (long)u * VE), v, p);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      sq = fmaf(v[i], v[i], sq);
-      big = fmaxf(big, fabsf(v[i]));
-    }
-  }
-  return guard_norm(wave_sum(sq), wave_max(big));
 }
 
 // the experts' counts of pairs, for the choice that follows
@@ -116,9 +93,11 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
   }
 }
 
-// The same by matrix cores: a workgroup per 64 router rows x 64 tokens, both kinds
-// of rows in LDS (128 k of each at a time, units exchanged as in wgemm.h), a wave
-// per 16 x 32. norms: |R[r]|^2, by the last workgroups.
+// The same by matrix cores: a workgroup per 64 router rows x 64 tokens (those of the
+// same tokens on one XCD, whose L2 then reads them once), both kinds of rows in LDS
+// (128 k of each at a time, units exchanged as in wgemm.h), a wave per 16 x 32.
+// norms: |R[r]|^2, then |x[t]|^2, the diagonals of products of 16 rows with
+// themselves, by the first workgroups of a column or a row of tiles.
 constexpr int LG_ROWS = 128;
 template <typename T> constexpr int LG_S = sizeof(T) == 2 ? 4 : 2;
 
@@ -129,14 +108,9 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   extern __shared__ __attribute__((aligned(16))) char s_buf[];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
-  const int e0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-  if (blockIdx.y == gridDim.y - 1) {                         // the router rows' norms
-    for (int r = e0 + wid; r < min(e0 + 64, A.cols); r += 8) {
-      const float n = row_norm(router_row(A, r), A.hidden, lane);
-      if (lane == 0) norms[r] = n;
-    }
-    return;
-  }
+  const int et = (A.cols + 63) / 64, item = xcd_run(blockIdx.x, gridDim.x);
+  const int e0 = item % et * 64, t0 = item / et * 64;
+  const bool w_norm = item < et && (wid & 1) == 0, x_norm = e0 == 0 && wid < 2;
   const T* src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -158,6 +132,9 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   for (int j = 0; j < S - 1; ++j)
     if (j < spans) fetch(j);
   double acc[2][4];
+  f32x4_t gram[3];                                           // of the router rows, of the tokens
+#pragma unroll
+  for (int u = 0; u < 3; ++u) gram[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -186,6 +163,27 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
+    if (w_norm) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) gram[0] = mma_piece(a[s], a[s], gram[0]);
+    }
+    if (x_norm) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) gram[1 + u] = mma_piece(b[s][u], b[s][u], gram[1 + u]);
+    }
+  }
+  // a wave's lane holds rows 4 g4 + i of column r16
+  if ((r16 >> 2) == g4) {
+    auto diagonal = [&](const f32x4_t& g) { return (r16 & 2) ? (r16 & 1) ? g[3] : g[2] : (r16 & 1) ? g[1] : g[0]; };
+    const int r = e0 + (wid >> 1) * 16 + r16;
+    if (w_norm && r < A.cols) norms[r] = diagonal(gram[0]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = t0 + (wid & 1) * 32 + 16 * u + r16;
+      if (x_norm && t < A.rows) norms[A.cols + t] = diagonal(gram[1 + u]);
+    }
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -207,10 +205,10 @@ struct TopArgs {
   const float* norms;  // null: the logits are sums in double already
 };
 
-// The logits of four experts in double, by the wave: lane c < 4 gets expert c's. One
-// round trip for all of them; the lanes' partial sums meet in the order of their
-// numbers' bits, whichever four are asked for.
-constexpr int EXACT = 4;
+// The logits of two experts in double (a close pair, mostly), by the wave: lane c < 2
+// gets expert c's. One round trip for both; the lanes' partial sums meet in the order
+// of their numbers' bits, whichever two are asked for.
+constexpr int EXACT = RT_EXACT;
 template <typename T>
 __device__ __forceinline__ double exact_logits(const QmLogits<T>& A, int t, const int (&e)[EXACT], int lane) {
   constexpr int VE = 16 / sizeof(T), B = 4;                  // units of a lane in flight
@@ -349,7 +347,7 @@ __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P,
   double off = 0.0;                        // the logits' own error
   bool all = false;                        // every logit has to be summed again
   if (P.norms) {
-    const float xn = row_norm(A.x + (long)t * A.ldx, A.hidden, lane);
+    const float xn = P.norms[A.cols + t];
     float wn = 0.f;
     bool bad = false;
 #pragma unroll
@@ -361,20 +359,31 @@ __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P,
       bad |= !(v < INFINITY) || !(fabs(l[e]) < (double)INFINITY);
     }
     wn = wave_max(wn);
-    // squares below float's range hide a norm
-    all = __builtin_amdgcn_ballot_w64(bad) != 0ull || !(xn < INFINITY) || (xn != 0.f && (xn < 0x1p-80f || wn < 0x1p-80f));
-    // (a row of zeros has logits of zero; the norms' own rounding is far below 2^-10)
-    if (xn != 0.f) off = 129.0 * 0x1p-23 * (1.0 + 0x1p-10) * sqrt((double)xn * (double)wn) + A.hidden * 0x1p-126;
+    // squares below float's range hide a norm: a row of zeros is looked through
+    bool zero = false;
+    if (xn < 0x1p-80f) {
+      constexpr int VE = 16 / sizeof(T);
+      unsigned any = 0u;
+      for (int u = lane; u < A.hidden / VE; u += 64) {
+        const uint4 v = *reinterpret_cast<const uint4*>(A.x + (long)t * A.ldx + (long)u * VE);
+        any |= (v.x | v.y | v.z | v.w) & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu);
+      }
+      zero = __builtin_amdgcn_ballot_w64(any != 0u) == 0ull;
+    }
+    all = __builtin_amdgcn_ballot_w64(bad) != 0ull || !(xn < INFINITY) || (!zero && (xn < 0x1p-80f || wn < 0x1p-80f));
+    // (its logits are zero; a norm's own sum is off by at most a step each time)
+    if (!zero)
+      off = 129.0 * 0x1p-23 * (1.0 + A.hidden * 0x1p-22) * sqrt((double)xn * (double)wn) + A.hidden * 0x1p-126;
   }
   long long key;                           // lane j: the j-th largest
   int id;
   if (!all)
     all = !wave_topk<PER>(l, A.experts, P.top_k, off, lane, key, id,
-                          [&](const int (&e)[4]) { return exact_logits(A, t, e, lane); });
+                          [&](const int (&e)[EXACT]) { return exact_logits(A, t, e, lane); });
   if (all) {
     if (P.norms) {
       for (int e0 = 0; e0 < A.experts; e0 += EXACT) {
-        const int last = A.experts - 1, e[EXACT] = {e0, min(e0 + 1, last), min(e0 + 2, last), min(e0 + 3, last)};
+        const int last = A.experts - 1, e[EXACT] = {e0, min(e0 + 1, last)};
         const double s = exact_logits(A, t, e, lane);
         if (lane < EXACT && e0 + lane < A.experts) l[e0 + lane] = s;
       }
@@ -426,7 +435,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 }  // namespace
 
-size_t qm_route_norms(int experts) { return ((size_t)experts + 1) * sizeof(float); }
+size_t qm_route_norms(int rows, int experts) { return ((size_t)rows + experts + 1) * sizeof(float); }
 
 template <typename T>
 int qm_route_logits(const QmLogits<T>& A, hipStream_t stream) {
@@ -447,7 +456,7 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
     const size_t lds = (size_t)LG_S<T> * LG_ROWS * WT_K * sizeof(T);
     rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds);
     if (rc) return rc;
-    hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64, (A.rows + 63) / 64 + 1), dim3(512), lds, stream, A, norms);
+    hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64 * ((A.rows + 63) / 64)), dim3(512), lds, stream, A, norms);
     QM_CHECK_LAUNCH();
   }
   if (rc) return rc;
@@ -487,7 +496,7 @@ int qm_check_route(const char* what, int act_dtype, int rows, int hidden, int ex
 
 extern "C" size_t qm_moe_route_workspace(int rows, int experts) {
   if (rows <= 0 || experts <= 0 || experts > RT_MAX_EXPERTS) return 0;
-  return qm_align256((size_t)rows * experts * sizeof(double)) + qm_align256(qm_route_norms(experts));
+  return qm_align256((size_t)rows * experts * sizeof(double)) + qm_align256(qm_route_norms(rows, experts));
 }
 
 extern "C" int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, int normalize, const void* x,
