@@ -330,6 +330,38 @@ def test_graph_replays(gpu, t):
             assert torch.equal(out, y) and torch.equal(ids, gpu.moe_route(x, args["router"], 4)[0])
 
 
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t,e,k,h,i", [(1, 16, 8, 256, 1536), (4, 64, 8, 544, 480), (13, 40, 6, 2048, 288)])
+def test_output_tiles_of_two_workgroups(gpu, fmt, t, e, k, h, i):
+    """Few tokens whose down products are long: two workgroups an output tile, the
+    last of which adds. Repeated, on two streams at once, and replayed."""
+    w, args = layer(gpu, t + i, e, h, i, 1, k, fmt, BF16)
+    xs = [normal(70 + s, t, h, dtype=BF16) for s in range(3)]
+    want = [gpu.moe(x, w) for x in xs]
+    for x, y in zip(xs, want):
+        check(y, x, args)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(gpu.moe(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[n % 2]) for n, y in enumerate(got))
+    static = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gpu.moe(static, w)
+    for x, y in zip(xs, want):
+        static.copy_(x)
+        graph.replay()
+        gpu.moe(xs[0], w)
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+
+
 def test_refusals(gpu):
     r = normal(1, 8, 64, dtype=BF16)
     gate, up, down = normal(2, 8, 32, 64, dtype=BF16), normal(3, 8, 32, 64, dtype=BF16), normal(4, 8, 64, 32, dtype=BF16)

@@ -74,6 +74,9 @@ struct FewArgs {
   int* slot_expert;    // [slot] expert; of a shared one -1 - its number
   int* slot_pair;      // [slot][16] the pair of each column, -1 where none
   float* slot_w;       // [slot][16] its weight
+  int split;           // workgroups of an output tile in the down products
+  float* down_part;    // [output tile][split][16 outputs][16] their sums
+  unsigned* down_done; // [output tile] how many have theirs there, cleared before
 };
 
 // choice `lane` of a token and its weight, by one wave
@@ -95,6 +98,11 @@ __device__ __forceinline__ int wave_choose(const double* l, int experts, int top
 }
 template <typename T> __device__ __forceinline__ float shared_weight(const FewArgs<T>& A, int t) {
   return A.cols > A.m.experts ? sigmoid_f((float)A.logits[(long)t * A.cols + A.m.experts]) : 1.f;
+}
+
+template <typename T> __device__ __forceinline__ void clear_down(const FewArgs<T>& A, int i, int threads) {
+  if (A.split > 1)
+    for (; i < wt_row_tiles(A.m.hidden); i += threads) A.down_done[i] = 0u;
 }
 
 // The table of slots, by one workgroup with a wave per token
@@ -120,6 +128,7 @@ __global__ __launch_bounds__(64 * FEW) void moe_few_plan_kernel(FewArgs<T> A) {
   // every column of every slot none, before the choices fill theirs
   const int most = M.shared + min(M.rows * M.top_k, M.experts);
   for (int i = threadIdx.x; i < most * 16; i += 64 * FEW) A.slot_pair[i] = -1;
+  clear_down(A, threadIdx.x, 64 * FEW);
   __syncthreads();
   if (threadIdx.x == 0) {
     int n = M.shared;
@@ -182,6 +191,7 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
       A.slot_pair[slot * 16 + threadIdx.x] = pair;
       if (threadIdx.x == 0) A.slot_expert[slot] = e;
       if (threadIdx.x == 0 && slot == 0) *A.n_slots = gridDim.y;
+      if (slot == 0) clear_down(A, threadIdx.x, 16);
     }
   } else {
     if (slot >= *A.n_slots) return;
@@ -231,7 +241,9 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
   store_act4(M.h + (long)pair * M.inter + n, v);
 }
 
-// out: a workgroup per 16 outputs; the waves share the (slot, k tile) units
+// out: a workgroup per 16 outputs, or `split` of them; the waves share the (slot,
+// k tile) units. Of several workgroups the last to finish adds their sums, in the
+// order of their numbers.
 template <typename WF, typename T>
 __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<T> A) {
   using F = Fmt<WF, T>;
@@ -242,11 +254,12 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
   const int kt = wt_k_tiles(M.inter), rt = wt_row_tiles(M.hidden);
-  const int units = *A.n_slots * kt;
+  const int units = *A.n_slots * kt, stride = NW * A.split, first = NW * blockIdx.y + wid;
   f32x4_t total = {0.f, 0.f, 0.f, 0.f};
   // a batch's slots are looked up while the one before is multiplied
   int expert[U], pair[U], at[U];
-  int slot = wid / kt, ks = wid % kt;                        // of the next unit to look up
+  int slot = first / kt, ks = first % kt;                    // of the next unit to look up
+  const int slot_step = stride / kt, ks_step = stride % kt;
   const int last = units / kt - 1;
   auto look_up = [&]() {
 #pragma unroll
@@ -255,13 +268,13 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
       expert[p] = A.slot_expert[s];
       pair[p] = A.slot_pair[s * 16 + r16];
       at[p] = ks;
-      slot += NW / kt;
-      ks += NW % kt;
+      slot += slot_step;
+      ks += ks_step;
       if (ks >= kt) { ks -= kt; ++slot; }
     }
   };
   look_up();
-  for (int u0 = wid; u0 < units; u0 += NW * U) {
+  for (int u0 = first; u0 < units; u0 += stride * U) {
     typename F::W w[U][1];
     Acts<F, T> x[U][1];
     bool mine[U];
@@ -277,7 +290,7 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
     look_up();
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      if (u0 + p * NW >= units) continue;
+      if (u0 + p * stride >= units) continue;
       f32x4_t acc[1][1];
       clear(acc);
       step_tile<F, T>(acc, w[p], x[p]);
@@ -288,12 +301,26 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
   }
   s_red[wid][lane] = total;
   __syncthreads();
-  if (wid != 0 || r16 >= M.rows) return;
+  if (wid != 0) return;
   f32x4_t v = s_red[0][lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) v += s_red[w][lane];
+  if (A.split > 1) {
+    float* parts = A.down_part + ((long)blockIdx.x * A.split * 64 + lane) * 4;
+    unsigned* mine = reinterpret_cast<unsigned*>(parts + blockIdx.y * 256);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st_flag(mine + i, __float_as_uint(v[i]));
+    wait_all_memory();                                       // the wave's stores, before they are counted
+    unsigned before = 0u;
+    if (lane == 0) before = __hip_atomic_fetch_add(A.down_done + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if ((int)__builtin_amdgcn_readfirstlane(before) != A.split - 1) return;
+    v = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < A.split; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(ld_flag(reinterpret_cast<const unsigned*>(parts + p * 256) + i));
+  }
   const int n = blockIdx.x * 16 + 4 * g4;
-  if (n < M.hidden) store_act4(M.out + (long)r16 * M.hidden + n, v);
+  if (r16 < M.rows && n < M.hidden) store_act4(M.out + (long)r16 * M.hidden + n, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -426,7 +453,7 @@ __global__ __launch_bounds__(256) void tile_weight_kernel(int n, int k, int rt, 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct MoeLayout {
-  size_t logits, norms, ids, pair_w, counts, lists, meta, tiles, h, part, bytes;
+  size_t logits, norms, ids, pair_w, counts, lists, meta, tiles, h, part, done, bytes;
   long max_tiles;      // of row tiles of bm rows
   int bm;
 };
@@ -448,6 +475,15 @@ int rows_per_tile(const qm_moe_geom& g) {
   if (mx) return avg < 512 ? 32 : 64;
   return avg < 40 ? 32 : avg < 128 ? 64 : 128;
 }
+// Workgroups of an output tile in the few tokens' down products: two where the tiles
+// alone leave half of the CUs without one and a wave has some six units of work (us,
+// 8 of 128 experts of 2048 x 512, with one / two: 4-bit 2 tokens 6.3 / 8.0, 3 tokens
+// 9.5 / 8.0, 9 tokens 15.2 / 11.2; bf16 9 tokens 29.6 / 24.8; 4096 x 1024, 256
+// tiles, 8 tokens 32.6 / 39.0; four are slower everywhere)
+int down_split(const qm_moe_geom& g) {
+  const long choices = (long)g.rows * g.top_k, slots = g.shared + (choices < g.experts ? choices : g.experts);
+  return wt_row_tiles(g.hidden) <= 128 && slots * wt_k_tiles(g.inter) >= 6 * FEW_DOWN_NW ? 2 : 1;
+}
 // The few-token kernels take the table of slots where the others keep the lists.
 MoeLayout moe_layout(const qm_moe_geom& g) {
   const size_t es = g.act_dtype == QM_ACT_BF16 ? 2 : 4;
@@ -463,6 +499,9 @@ MoeLayout moe_layout(const qm_moe_geom& g) {
     l.counts = take((g.shared + hot) * sizeof(int));          // slot_expert
     l.lists = take((g.shared + hot) * 16 * sizeof(int));      // slot_pair
     l.pair_w = take((g.shared + hot) * 16 * sizeof(float));   // slot_w
+    const size_t split = down_split(g);
+    l.part = take(split > 1 ? wt_row_tiles(g.hidden) * split * 256 * sizeof(float) : 0);
+    l.done = take(split > 1 ? wt_row_tiles(g.hidden) * sizeof(unsigned) : 0);
   } else {
     l.bm = rows_per_tile(g);
     // every expert's last tile may be part-filled
@@ -547,7 +586,7 @@ int launch_few_per(const FewArgs<T>& A, int max_slots, hipStream_t stream) {
                        stream, A);
   }
   QM_CHECK_LAUNCH();
-  hipLaunchKernelGGL((moe_few_down_kernel<WF, T>), dim3(wt_row_tiles(A.m.hidden)), dim3(64 * FEW_DOWN_NW), 0, stream, A);
+  hipLaunchKernelGGL((moe_few_down_kernel<WF, T>), dim3(wt_row_tiles(A.m.hidden), A.split), dim3(64 * FEW_DOWN_NW), 0, stream, A);
   QM_CHECK_LAUNCH();
   return QM_OK;
 }
@@ -583,7 +622,8 @@ int run_moe(const qm_moe_geom& g, const qm_moe_weights& w, const void* x, long l
   A.out = static_cast<T*>(out);
   if (g.rows <= FEW) {
     const FewArgs<T> P = {A, L.logits, L.cols, g.normalize, meta, counts,
-                          reinterpret_cast<int*>(ws + l.lists), reinterpret_cast<float*>(ws + l.pair_w)};
+                          reinterpret_cast<int*>(ws + l.lists), reinterpret_cast<float*>(ws + l.pair_w), down_split(g),
+                          reinterpret_cast<float*>(ws + l.part), reinterpret_cast<unsigned*>(ws + l.done)};
     const int rc = qm_route_logits(L, stream);
     if (rc) return rc;
     return mx ? launch_few<WMx4, T>(P, stream) : launch_few<WPlain, T>(P, stream);
