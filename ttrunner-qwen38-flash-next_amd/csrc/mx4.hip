@@ -159,9 +159,11 @@ __global__ __launch_bounds__(MX_NT) void mx4_layout_kernel(MxGeom g, uint8_t* co
 
 // ---------------------------------------------------------------------------
 // y[m][n] = sum_k W[n][k] x[m][k] for a few activation rows: a stream over the
-// weights. A workgroup takes TN row tiles against MT tiles of 16 activation
-// rows, its waves split the k tiles (PS of them in flight at a time), the partial
-// results meet in LDS. Every weight is loaded once per 16 MT rows.
+// weights. A workgroup takes TN row tiles against a tile of 16 activation rows, its
+// waves split the k tiles, the partial results meet in LDS. Every weight is loaded once per 16 rows. A wave's activations go through
+// its own part of LDS: straight from memory their operand would take each lane of a
+// load from another row than its neighbour, and such a load costs a cycle a lane
+// (bf16, 12352 x 2048: 16 rows 7.4 us so, 5.7 through LDS; 1 row 5.0 and 5.2).
 template <typename T>
 struct Mx4LinearArgs {
   WMat w;
@@ -191,47 +193,52 @@ __device__ __forceinline__ void store4(const Mx4LinearArgs<T>& A, int m, int n, 
   }
 }
 
-template <typename T, int TN, int MT, int NW, int PS>
+template <typename T, int TN, int NW>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4LinearArgs<T> A) {
   using F = Fmt<WMx4, T>;
-  __shared__ f32x4_t s_red[NW][TN * MT][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  constexpr int ROW_B = WT_K * sizeof(T), UNITS = ROW_B / 16, VE = 16 / sizeof(T), RPL = 1024 / ROW_B;
+  constexpr int X_B = 16 * ROW_B;
+  __shared__ __attribute__((aligned(16))) char s_buf[NW * (X_B > TN * 1024 ? X_B : TN * 1024)];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
-  const int t0 = blockIdx.x * TN, m0 = blockIdx.y * 16 * MT;
-  f32x4_t acc[TN][MT];
+  const int t0 = blockIdx.x * TN, m0 = blockIdx.y * 16, rows = min(16, A.m - m0);
+  char* s_x = s_buf + wid * X_B;                             // 16 rows, units exchanged as in wgemm.h
+  f32x4_t acc[TN][1];
   clear(acc);
-  for (int k0 = wid; k0 < A.kt; k0 += NW * PS) {
-    typename F::W w[PS][TN];
-    Acts<F, T> x[PS][MT];
+  for (int ks = wid; ks < A.kt; ks += NW) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the rows before are read
 #pragma unroll
-    for (int p = 0; p < PS; ++p) {
-      const int ks = min(k0 + p * NW, A.kt - 1);
-#pragma unroll
-      for (int t = 0; t < TN; ++t) w[p][t] = F::load_w(A.w, (long)min(t0 + t, A.rt - 1) * A.kt + ks, lane);
-#pragma unroll
-      for (int u = 0; u < MT; ++u) x[p][u].load(A.x + (long)min(m0 + 16 * u + r16, A.m - 1) * A.ldx, ks, A.k, g4);
+    for (int q = 0; q < 16 / RPL; ++q) {
+      if (q * RPL >= rows) continue;                         // (rows past the last multiply what lies there, unread)
+      const int row = q * RPL + lane / UNITS, k = ks * WT_K + ((lane % UNITS) ^ row) * VE;
+      const T* src = A.x + (long)min(m0 + row, A.m - 1) * A.ldx + k;
+      lds_load16(k < A.k ? static_cast<const void*>(src) : g_zero_unit, s_x + q * 1024);
     }
+    typename F::W w[TN];
+    Acts<F, T> x[1];
 #pragma unroll
-    for (int p = 0; p < PS; ++p)
-      if (k0 + p * NW < A.kt) step_tile<F, T>(acc, w[p], x[p]);
+    for (int t = 0; t < TN; ++t) w[t] = F::load_w(A.w, (long)min(t0 + t, A.rt - 1) * A.kt + ks, lane);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // this wave's rows are in LDS
+#pragma unroll
+    for (int s = 0; s < 4; ++s) x[0].p[s] = lds_piece<T>(s_x + r16 * ROW_B, F::unit(g4, s), r16);
+    step_tile<F, T>(acc, w, x);
   }
+  __syncthreads();                                           // the sums take the rows' place
+  f32x4_t (*s_red)[TN][64] = reinterpret_cast<f32x4_t (*)[TN][64]>(s_buf);
 #pragma unroll
-  for (int t = 0; t < TN; ++t)
-#pragma unroll
-    for (int u = 0; u < MT; ++u) s_red[wid][t * MT + u][lane] = acc[t][u];
+  for (int t = 0; t < TN; ++t) s_red[wid][t][lane] = acc[t][0];
   __syncthreads();
-  for (int r = wid; r < TN * MT; r += NW) {
+  for (int r = wid; r < TN; r += NW) {
     f32x4_t v = s_red[0][r][lane];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += s_red[w][r][lane];
-    store4(A, m0 + 16 * (r % MT) + r16, (t0 + r / MT) * 16 + 4 * g4, v);
+    store4(A, m0 + r16, (t0 + r) * 16 + 4 * g4, v);
   }
 }
 
-template <typename T, int TN, int MT, int NW, int PS>
+template <typename T, int TN, int NW>
 int launch_rows(const Mx4LinearArgs<T>& A, hipStream_t stream) {
-  hipLaunchKernelGGL((mx4_rows_kernel<T, TN, MT, NW, PS>),
-                     dim3((A.rt + TN - 1) / TN, (A.m + 16 * MT - 1) / (16 * MT)), dim3(64 * NW), 0, stream, A);
+  hipLaunchKernelGGL((mx4_rows_kernel<T, TN, NW>), dim3((A.rt + TN - 1) / TN, (A.m + 15) / 16), dim3(64 * NW), 0, stream, A);
   QM_CHECK_LAUNCH();
   return QM_OK;
 }
@@ -274,36 +281,46 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   return QM_OK;
 }
 
-// The kernel for m rows (weights from memory, graph replays, us a call):
-//   bf16, up to 16 rows   two row tiles a workgroup where the weight has 256 of them
-//     or more (12352 x 2048: 1 row 5.0, 16 rows 7.3, with one tile 5.4 and 10.2),
-//     else one, two k tiles a wave in flight (2048 x 4096: 1 row 3.9, 14 rows 6.0,
-//     with two tiles 4.5 and 6.4)
-//   bf16, more rows   the largest of the tiles of wgemm.h that makes 256 workgroups
-//     (160 for the smallest). 12352 x 2048, 256 x 64 / 256 x 32 / 128 x 32 / 128 x 16
-//     tiles: 64 rows 20.2 / 13.9 / 11.7 / 10.6, 128 rows 20.5 / 14.4 / 13.8 / 18.1,
-//     256 rows 21.2 / 20.1 / 25.6 / 26.8, 512 rows 33.1 / 37.3 / 39.8 / 50. Fewer
-//     workgroups than that: the few-row kernel with k split over 16 waves (2048 x
-//     4096: 64 rows 7.1 against 14.4, 128 rows 12.1 against 14.5)
-//   float   the same with the smallest tile alone (its activations are cut into
-//     parts by every workgroup: 12352 x 2048, 64 rows 31 against 37 with 32 rows a
-//     tile, 256 rows 88 against 99)
+// The kernel for m rows (weights from memory, graph replays, us a call). g(TN) is the
+// number of workgroups of the few-row kernel with TN row tiles each.
+//   few rows   up to one workgroup a CU, k is split over 16 waves (2048 x 4096, 64
+//     rows: 16 waves 5.2, 8 waves 5.5); more of them keep 8 (12352 x 2048, one row:
+//     5.1 against 6.2). Of bf16 a workgroup takes one row tile while there is one a
+//     CU (2048 x 4096, 16 rows: 1, 2, 4 tiles 4.5 / 5.3 / 6.7; 64 rows 7.5 / 5.6 /
+//     6.9), two while there are two (12352 x 2048, 16 rows: 7.0 / 5.6 / 5.7), else
+//     four (256 rows of 2048 x 4096: - / 11.8 / 10.5). Floats are cut into parts by
+//     every workgroup, so as many tiles as leave one a CU share them, up to eight
+//     (12352 x 2048, 1 row: 1, 2, 4, 8 tiles 12.5 / 8.7 / 7.6 / 10; 32 rows 22 / 16 /
+//     12.0 / 11.5).
+//   bf16, more than 640 of them with four tiles each   the largest of the tiles of
+//     wgemm.h that makes 256 workgroups, else the smallest. 12352 x 2048, few-row
+//     kernel / 128 x 16 / 128 x 32 / 256 x 32 / 256 x 64: 48 rows (579) 10.5 / 10.6 /
+//     12.0 / 13.8 / 19.6, 64 rows (772) 12.7 / 10.4 / 11.9 / 14.1 / 20.5, 128 rows
+//     20.1 / 17.9 / 14.2 / 14.5 / 20.6, 200 rows 28.9 / 21.1 / 18.2 / 20.2 / 21.4; at
+//     2048 x 4096, whose k is longer, the few-row kernel leads up to 512 rows (1024:
+//     17.2 / 18.5)
+//   float   256 x 32 tiles from 512 workgroups on (2000 rows of 9856 x 2048: 283
+//     against 328; 256 of 12352 x 2048, 392 of them: 60 against 63)
 template <typename T>
 int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   auto groups = [&A](int bn, int bm) { return (long)((A.rt * 16 + bn - 1) / bn) * ((A.m + bm - 1) / bm); };
-  if (A.m <= 16) {
-    if (A.rt >= 256) return launch_rows<T, 2, 1, 8, 1>(A, stream);
-    return launch_rows<T, 1, 1, 8, 2>(A, stream);
-  }
   if constexpr (sizeof(T) == 2) {
-    if (groups(256, 64) >= 256) return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
-    if (groups(256, 32) >= 256) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
-    if (groups(128, 32) >= 256) return launch_gemm<T, 2, 2, 4, 1, 3>(A, stream);
-    if (groups(128, 16) >= 160) return launch_gemm<T, 2, 1, 4, 1, 4>(A, stream);
-    return launch_rows<T, 2, 1, 16, 1>(A, stream);
+    if (groups(64, 16) > 640) {
+      if (groups(256, 64) >= 256) return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
+      if (groups(256, 32) >= 256) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
+      if (groups(128, 32) >= 256) return launch_gemm<T, 2, 2, 4, 1, 3>(A, stream);
+      return launch_gemm<T, 2, 1, 4, 1, 4>(A, stream);
+    }
+    if (groups(16, 16) <= 256) return launch_rows<T, 1, 16>(A, stream);
+    if (groups(32, 16) <= 256) return launch_rows<T, 2, 16>(A, stream);
+    if (groups(32, 16) <= 512) return launch_rows<T, 2, 8>(A, stream);
+    return launch_rows<T, 4, 8>(A, stream);
   } else {
-    if (groups(128, 16) >= 256) return launch_gemm<T, 2, 1, 4, 1, 3>(A, stream);
-    return launch_rows<T, 2, 1, 8, 1>(A, stream);
+    if (groups(256, 32) >= 512) return launch_gemm<T, 4, 2, 4, 1, 2>(A, stream);
+    if (groups(16, 16) <= 256) return launch_rows<T, 1, 16>(A, stream);
+    if (groups(32, 16) <= 256) return launch_rows<T, 2, 16>(A, stream);
+    if (groups(64, 16) <= 256) return launch_rows<T, 4, 8>(A, stream);
+    return launch_rows<T, 8, 8>(A, stream);
   }
 }
 
