@@ -61,36 +61,64 @@ template <typename T> __device__ __forceinline__ void clear_counts(const QmLogit
     for (int i = threadIdx.x; i <= A.experts; i += blockDim.x) A.counts[i] = 0;
 }
 
-// logits[t][r] of the router's rows and, when there is one, the shared experts' row
-template <typename T>
+// logits[t][r] of the router's rows and, when there is one, the shared experts' row:
+// a wave per router row and TB tokens
+template <typename T, int TB>
 __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
-  constexpr int VE = 16 / sizeof(T);
+  constexpr int VE = 16 / sizeof(T), B = TB == 1 ? 4 : 2;    // units of a lane in flight
   const int lane = threadIdx.x & 63;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   clear_counts(A);
   if (r >= A.cols) return;
-  const int t0 = blockIdx.y * RT_TB;
+  const int t0 = blockIdx.y * TB, units = A.hidden / VE;
   const T* w = router_row(A, r);
-  double acc[RT_TB];
+  const T* x[TB];
+  double acc[TB];
 #pragma unroll
-  for (int i = 0; i < RT_TB; ++i) acc[i] = 0.0;
-  for (int u = lane; u < A.hidden / VE; u += 64) {
-    float wv[VE];
-    unit_get(*reinterpret_cast<const uint4*>(w + (long)u * VE), wv, w);
+  for (int i = 0; i < TB; ++i) {
+    x[i] = A.x + (long)min(t0 + i, A.rows - 1) * A.ldx;
+    acc[i] = 0.0;
+  }
+  for (int u0 = lane; u0 < units; u0 += 64 * B) {
+    uint4 wu[B], xu[B][TB];
 #pragma unroll
-    for (int i = 0; i < RT_TB; ++i) {
-      if (t0 + i >= A.rows) break;
-      float xv[VE];
-      unit_get(*reinterpret_cast<const uint4*>(A.x + (long)(t0 + i) * A.ldx + (long)u * VE), xv, w);
+    for (int b = 0; b < B; ++b) {
+      const long at = (long)min(u0 + 64 * b, units - 1) * VE;
+      wu[b] = *reinterpret_cast<const uint4*>(w + at);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[i] = exact_fma(wv[e], xv[e], acc[i]);
+      for (int i = 0; i < TB; ++i) xu[b][i] = *reinterpret_cast<const uint4*>(x[i] + at);
+    }
+    __builtin_amdgcn_sched_barrier(0);                       // all of them in flight
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (u0 + 64 * b >= units) break;
+      float wv[VE];
+      unit_get(wu[b], wv, w);
+#pragma unroll
+      for (int i = 0; i < TB; ++i) {
+        float xv[VE];
+        unit_get(xu[b][i], xv, w);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[i] = exact_fma(wv[e], xv[e], acc[i]);
+      }
     }
   }
+  // the lanes' sums meet in the order of their numbers' bits, as in exact_logits; of
+  // four tokens half a wave, then a quarter goes on with its own
+  int t = t0;
+  if constexpr (TB == 4) {
 #pragma unroll
-  for (int i = 0; i < RT_TB; ++i) {
-    const double s = lanes_sum_f64<64>(acc[i]);
-    if (lane == 0 && t0 + i < A.rows) A.logits[(long)(t0 + i) * A.cols + r] = s;
+    for (int i = 0; i < 2; ++i) {
+      const double give = lane & 32 ? acc[i] : acc[i + 2];
+      acc[i] = (lane & 32 ? acc[i + 2] : acc[i]) + __shfl_xor(give, 32, 64);
+    }
+    const double give = lane & 16 ? acc[0] : acc[1];
+    acc[0] = lanes_sum_f64<16>((lane & 16 ? acc[1] : acc[0]) + __shfl_xor(give, 16, 64));
+    t += (lane >> 4 & 1) + (lane >> 4 & 2);
+  } else {
+    acc[0] = lanes_sum_f64<64>(acc[0]);
   }
+  if ((TB == 4 ? lane & 15 : lane) == 0 && t < A.rows) A.logits[(long)t * A.cols + r] = acc[0];
 }
 
 // The same by matrix cores: a workgroup per 64 router rows x 64 tokens (those of the
@@ -439,7 +467,8 @@ size_t qm_route_norms(int rows, int experts) { return ((size_t)rows + experts + 
 
 template <typename T>
 int qm_route_logits(const QmLogits<T>& A, hipStream_t stream) {
-  hipLaunchKernelGGL(moe_logits_kernel<T>, dim3((A.cols + 3) / 4, (A.rows + RT_TB - 1) / RT_TB), dim3(256), 0, stream, A);
+  if (A.rows == 1) hipLaunchKernelGGL((moe_logits_kernel<T, 1>), dim3((A.cols + 3) / 4), dim3(256), 0, stream, A);
+  else hipLaunchKernelGGL((moe_logits_kernel<T, RT_TB>), dim3((A.cols + 3) / 4, (A.rows + RT_TB - 1) / RT_TB), dim3(256), 0, stream, A);
   QM_CHECK_LAUNCH();
   return QM_OK;
 }
