@@ -60,8 +60,11 @@ def linear(x, w):
 
 
 def route(x, router, top_k, normalize=True):
-    """(ids, weights): equal logits to the lower index."""
-    logits = x.double() @ router.double().t()
+    """(ids, weights): equal logits to the lower index. Equal router rows are
+    multiplied once: a library's product may sum their columns in different orders,
+    and its last bits would order what is equal."""
+    rows, which = torch.unique(router.double(), dim=0, return_inverse=True)
+    logits = (x.double() @ rows.t())[:, which]
     order = logits.sort(dim=-1, descending=True, stable=True).indices[:, :top_k]
     w = torch.softmax(logits, -1).gather(1, order)
     return order.int(), w / w.sum(-1, keepdim=True) if normalize else w

@@ -94,7 +94,8 @@ MANY = [(500, 130, 8, 2080), (130, 1024, 32, 1056), (1700, 60, 4, 1024), (3300, 
 @pytest.mark.parametrize("t,e,k,h", MANY)
 @pytest.mark.parametrize("normalize", [True, False])
 def test_route_many_rows(gpu, dtype, t, e, k, h, normalize):
-    assert t * e * h > 1e8
+    t = t if dtype == BF16 else 5 * t
+    assert t * e * h > (1e8 if dtype == BF16 else 4.5e8)
     x, r = normal(t + e, t, h, dtype=dtype), normal(h, e, h, dtype=dtype, scale=h ** -0.5)
     ids, w = gpu.moe_route(x, r, k, normalize)
     want_ids, want_w = fo.route(x, r, k, normalize)
@@ -116,7 +117,7 @@ def test_route_many_rows(gpu, dtype, t, e, k, h, normalize):
 @pytest.mark.parametrize("copies", [3, 40, 150])
 def test_route_many_rows_close_logits(gpu, dtype, copies):
     """Router rows a last bit apart (the order takes sums in double) and equal ones."""
-    t, e, h, k = 600, 160, 1184, 12
+    t, e, h, k = 600 if dtype == BF16 else 2600, 160, 1184, 12
     x = normal(1, t, h, dtype=dtype)
     r = normal(2, e, h, dtype=dtype, scale=h ** -0.5)
     near = torch.randperm(e, generator=torch.Generator().manual_seed(3))[:copies].tolist()
@@ -133,7 +134,7 @@ def test_route_many_rows_close_logits(gpu, dtype, copies):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_route_many_rows_ties_magnitudes_and_bad_values(gpu, dtype):
-    t, e, h, k = 700, 96, 1632, 6
+    t, e, h, k = 700 if dtype == BF16 else 3100, 96, 1632, 6
     r = normal(2, e, h, dtype=dtype, scale=h ** -0.5)
     x = normal(1, t, h, dtype=dtype)
     x *= torch.logspace(-38, 17, t, device=DEV).to(dtype)[:, None]
@@ -145,8 +146,7 @@ def test_route_many_rows_ties_magnitudes_and_bad_values(gpu, dtype):
     assert torch.equal(ids, want) and ids[5].tolist() == list(range(k))
     assert bool((w.sum(-1) - 1).abs().max() < 2.0 ** -20) and bool((w[5] == w[5, 0]).all())
     small = normal(4, e, h, dtype=dtype, scale=1e-30)               # products below float's range
-    tiny_ids = gpu.moe_route(x[:400], small, k)[0] if 400 * e * h > 1e8 else gpu.moe_route(x, small, k)[0]
-    assert torch.equal(tiny_ids, fo.route(x, small, k)[0][:tiny_ids.shape[0]])
+    assert torch.equal(gpu.moe_route(x, small, k)[0], fo.route(x, small, k)[0])
     zero = torch.zeros_like(x)
     ids0, w0 = gpu.moe_route(zero, r, k)
     assert ids0.tolist() == [list(range(k))] * t and torch.equal(w0, torch.full_like(w0, w0[0, 0].item()))

@@ -20,7 +20,11 @@
 
 namespace {
 
-constexpr double ROUTE_FEW = 1e8;
+// Products of a call (rows x columns x hidden) up to which every logit is summed in
+// double. Logits and choice of 128 experts over 2048, us, so / by matrix cores: bf16
+// 256 rows (7e7) 18 / 24, 460 rows (1.2e8) 26 / 25, 1000 rows 46 / 26; float 1024
+// rows (2.7e8) 53 / 82, 1500 rows 74 / 84, 2048 rows (5.4e8) 98 / 83.
+template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 4.5e8;
 // Choices of an expert, on average, up to which the choosing waves file them by
 // atomics (they serialise: 8 each +2.4 us, 16 +4.2, 32 +7.2, 250 +31); beyond, a
 // launch of its own does (6.0 us and its start, 7.7 at 16000 choices)
@@ -478,7 +482,7 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
              const QmRouteLists* lists, float* norms, hipStream_t stream) {
   TopArgs P = {top_k, normalize, ld_w, shared, ids, weights, lists ? *lists : QmRouteLists{}, nullptr};
   int rc;
-  if ((double)A.rows * A.cols * A.hidden <= ROUTE_FEW) {
+  if ((double)A.rows * A.cols * A.hidden <= ROUTE_FEW<T>) {
     rc = qm_route_logits(A, stream);
   } else {
     P.norms = norms;
