@@ -219,10 +219,10 @@ def test_moe_matches_f64(gpu, dtype, fmt, t, e, k, h, i, shared):
 # weights read once; logits by matrix cores; the largest top_k, experts and shared
 @pytest.mark.parametrize("fmt", ["plain", "mx4"])
 @pytest.mark.parametrize("t,e,k,h,i,shared", [(16, 24, 4, 288, 160, 1), (17, 24, 4, 288, 160, 1), (300, 8, 2, 160, 96, 1),
-                                              (1100, 4, 2, 160, 96, 1), (3000, 32, 6, 64, 32, 0), (290, 24, 2, 96, 64, 0),
-                                              (280, 24, 2, 96, 64, 1), (1700, 60, 4, 1056, 32, 1), (16, 1024, 32, 32, 32, 1),
-                                              (40, 1024, 32, 32, 32, 0), (3, 32, 32, 64, 32, 32), (20, 32, 32, 64, 32, 32),
-                                              (16, 1, 1, 96, 32, 0), (90, 1, 1, 96, 32, 0)])
+                                              (300, 16, 2, 160, 96, 1), (1100, 4, 2, 160, 96, 1), (3000, 32, 6, 64, 32, 0),
+                                              (290, 24, 2, 96, 64, 0), (280, 24, 2, 96, 64, 1), (1700, 60, 4, 1056, 32, 1),
+                                              (16, 1024, 32, 32, 32, 1), (40, 1024, 32, 32, 32, 0), (3, 32, 32, 64, 32, 32),
+                                              (20, 32, 32, 64, 32, 32), (16, 1, 1, 96, 32, 0), (90, 1, 1, 96, 32, 0)])
 def test_moe_borders(gpu, fmt, t, e, k, h, i, shared):
     print(f"moe {fmt} t={t} e={e} k={k} h={h} i={i} shared={shared}", flush=True)
     w, args = layer(gpu, t + e, e, h, i, shared, k, fmt, BF16, normalize=t % 2 == 0)

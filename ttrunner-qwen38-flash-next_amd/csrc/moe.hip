@@ -61,6 +61,12 @@ __device__ __forceinline__ WMat expert_mat(const WMat& m, int e, long tiles, int
 // their numbers. A single token's workgroups rank its logits for themselves (a
 // launch of its own for that takes longer); for several tokens one workgroup
 // does and leaves the table of slots.
+//
+// What bounds it is the weights' way from memory. 8 of 128 experts of 2048 x 512 and
+// a shared one: one token, bf16, 57 MB: logits 3.0 us, up 10 to 11.5 (3 of them the
+// ranking), down 5.8; 9 tokens, 4-bit, 107 MB: 4.1, table 5.8, up 15 (4.7 TB/s), down
+// 11. Against the many-token kernels: 8 tokens, 4-bit, 35 for 40 us, 16 tokens 47 and
+// 47, bf16 100 for 110.
 // ---------------------------------------------------------------------------
 constexpr int FEW = 16;
 constexpr int FEW_UP_NW = 8, FEW_DOWN_NW = 16;
@@ -152,7 +158,11 @@ __global__ __launch_bounds__(64 * FEW) void moe_few_plan_kernel(FewArgs<T> A) {
   }
 }
 
-// h of a slot: a workgroup per 16 TN hidden units and slot, the waves split k
+// h of a slot: a workgroup per 16 TN hidden units and slot, the waves split k (a
+// wave's loads are whole lines of tiles; the partial results meet in LDS). TN: 4-bit
+// weights are few bytes beside the activations' operands, so two row tiles share
+// them (16 tokens of 8 of 128 experts, us with one / two: 4-bit 22.6 / 18.8, bf16
+// 54.8 / 61.2).
 template <typename WF, typename T, int PER, bool ONE, int TN>
 __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A) {
   using F = Fmt<WF, T>;
@@ -326,11 +336,16 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
 // ---------------------------------------------------------------------------
 // Many tokens: routing, the experts' lists of pairs, the up products, the down
 // products of every pair, and their sum per token.
+//
+// 2000 tokens, 8 of 64 experts of 2048 x 768 and a shared one, bf16: routing 33 us, up
+// 163, down 124, sum 25. The up products read 400 MB of weights and do 113 GFLOP (a
+// quarter more with the experts' last tiles filled up): 620 MB from behind the L2 at
+// 3.9 TB/s and 870 TFLOP/s at once, neither alone at its limit. 128 tokens, 4-bit, 8 of
+// 128 of 2048 x 512: up 30 us, down 19, the weights at 4.6 and 3.8 TB/s.
 // ---------------------------------------------------------------------------
-// The same over many rows (wgemm.h): a workgroup per row tile of the table and
-// range of weight rows, the ranges of a tile side by side on an XCD. Of a wave's
-// TN row tiles the first half are gate rows, the others the up rows of the same
-// hidden units.
+// A workgroup (wgemm.h) per row tile of the table and range of weight rows, the
+// ranges of a tile side by side on an XCD. Of a wave's TN row tiles the first half
+// are gate rows, the others the up rows of the same hidden units.
 template <typename WF, typename T, int TN, int TM, int WN, int WM, int S, bool STREAM>
 __global__ __launch_bounds__(64 * WN * WM, 2) void moe_up_gemm_kernel(MoeArgs<T> A) {
   using G = SpanGemm<WF, T, TN, TM, WN, WM, S, STREAM>;
@@ -406,7 +421,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void moe_down_gemm_kernel(MoeArgs<
 }
 
 // y[t] = the sum of its pairs' products, in their order (a thread per 16 bytes of
-// the output). The products stay in float: in bf16 their rounding would add as much
+// the output): a stream (2000 tokens of 9 pairs, 156 MB, 25 us). The products stay in float: in bf16 their rounding would add as much
 // error again as the hidden rows' (2000 tokens of 9 pairs: relative error 2.9e-3
 // for 2.4e-3, and 21 us of 339 saved).
 template <typename T>
@@ -428,7 +443,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs<T> A) {
   for (int e = 0; e < VE / 4; ++e) store_act4(A.out + t * A.hidden + c + 4 * e, v[e]);
 }
 
-// rows of bf16 or float weights into tiles (a wave per tile)
+// rows of bf16 or float weights into tiles (a wave per tile): once, when the weights
+// are made (128 experts of 2048 x 512, 268 MB there and back, 92 us)
 template <typename T>
 __global__ __launch_bounds__(256) void tile_weight_kernel(int n, int k, int rt, int kt, long tiles, const T* w, char* out) {
   constexpr int VE = 16 / sizeof(T), PIECES = 32 / VE;
@@ -459,21 +475,20 @@ struct MoeLayout {
 };
 
 // Activation rows of a tile of the many-token kernels, by the rows that an expert
-// has on average (us a layer, 8 experts of a token; tiles of 16 / 32 / 64 / 128
-// rows, the best shape of each):
-//   bf16 weights, 128 experts of 2048 x 512: 8 rows 175 / 174 / 178 / 183, 25 rows
-//     227 / 196 / 197 / 203, 62 rows 347 / 264 / 234 / 245; 64 of 2048 x 768: 250
-//     rows 806 / 464 / 343 / 322
-//   4-bit weights: 8 rows 84 / 79 / 98 / 182, 31 rows - / 118 / 122 / 205, 125 rows
-//     - / 231 / 236 / 303, 750 rows (2048 x 768) - / 742 / 710 / 897
-//   float activations, 25 rows: float weights 340 / 231 / 376, 4-bit ones 127 / 142
-//     / 308
+// has on average (us a layer, 8 experts of a token):
+//   bf16 weights, 128 experts of 2048 x 512, tiles of 32 / 64 / 128 rows: 8 rows 152 /
+//     169 / 170, 25 rows 206 / 195 / 204, 62 rows 262 / 234 / 228; 64 of 2048 x 768:
+//     250 rows 493 / 357 / 312
+//   4-bit weights, 32 / 64: 8 rows 67 / 82, 31 rows 109 / 112, 125 rows 209 / 212, 375
+//     rows (2048 x 768) 341 / 339, 750 rows 642 / 620
+//   float activations, 25 rows, 16 / 32: float weights 419 / 400, 4-bit ones 193 / 217;
+//     125 rows: 1308 / 1168, 614 / 677
 int rows_per_tile(const qm_moe_geom& g) {
   const double avg = (double)g.rows * g.top_k / g.experts;
   const bool mx = g.weight_format == QM_W_MX4;
   if (g.act_dtype != QM_ACT_BF16) return mx ? 16 : 32;
   if (mx) return avg < 512 ? 32 : 64;
-  return avg < 40 ? 32 : avg < 128 ? 64 : 128;
+  return avg < 20 ? 32 : avg < 48 ? 64 : 128;
 }
 // Workgroups of an output tile in the few tokens' down products: two where the tiles
 // alone leave half of the CUs without one and a wave has some six units of work (us,
@@ -574,7 +589,6 @@ int launch_ffn(const MoeArgs<T>& A, int bm, bool once, long max_tiles, hipStream
 
 template <typename WF, typename T, int PER>
 int launch_few_per(const FewArgs<T>& A, int max_slots, hipStream_t stream) {
-  // 4-bit weights are few bytes beside the activations' operands: two tiles share them
   constexpr int TN = Fmt<WF, T>::SCALED ? 2 : 1;
   const int rt = wt_row_tiles(A.m.inter);
   if (A.m.rows == 1) {
