@@ -11,6 +11,9 @@ the output's rounding are independent, each 0.58 half steps in the mean.
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -228,6 +231,18 @@ def test_moe_borders(gpu, fmt, t, e, k, h, i, shared):
     w, args = layer(gpu, t + e, e, h, i, shared, k, fmt, BF16, normalize=t % 2 == 0)
     x = normal(t, t, h, dtype=BF16)
     check(gpu.moe(x, w), x, args)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+def test_a_copied_layer_has_its_own_memory(gpu, fmt):
+    w, args = layer(gpu, 5, 6, 96, 64, 1, 2, fmt, BF16)
+    x = normal(6, 20, 96, dtype=BF16)
+    want = gpu.moe(x, w)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert torch.equal(gpu.moe(x, other), want)
+        for t in (other.down, other.s_down):
+            t.data.zero_()
+        assert not bool(gpu.moe(x, other).any()) and torch.equal(gpu.moe(x, w), want)
 
 
 @pytest.mark.parametrize("fmt", ["plain", "mx4"])

@@ -8,6 +8,9 @@ of half a step have 0.58 of it in the mean, so twice half a step is ample.
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -181,6 +184,37 @@ def test_linear_on_a_side_stream_and_in_a_graph(gpu):
         gpu.mx4_linear(x, q)                                        # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(out, w)
+
+
+def test_a_copied_and_a_saved_weight_have_their_own_memory(gpu):
+    q = gpu.mx4_quantize(normal(3, 40, 160, dtype=BF16))
+    x = normal(4, 5, 160, dtype=BF16)
+    want = gpu.mx4_linear(x, q)
+    for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert other.data.data_ptr() != q.data.data_ptr()
+        assert other.codes_ptr == other.codes.data_ptr() and other.scales_ptr == other.scales.data_ptr()
+        other.data.zero_()                                          # leaves the first alone
+        assert not bool(gpu.mx4_linear(x, other).any())
+        assert torch.equal(gpu.mx4_linear(x, q), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_with_subnormal_weights_and_activations(gpu, dtype, m):
+    """Scale byte 0 (elements from 2^-128) and activations below float's normal range."""
+    w = torch.zeros(64, 64, device=DEV)
+    w[torch.arange(64), torch.arange(64)] = 3 * 2.0 ** -127 if dtype == BF16 else 1.0
+    x = normal(5, m, 64, dtype=dtype)
+    if dtype == F32:
+        x *= 2.0 ** -120
+    q = gpu.mx4_quantize(w)
+    want = x.double() * q.dequantize().double().diagonal()
+    got = gpu.mx4_linear(x, q).double()
+    # One product a sum: the output's rounding, for bf16 a step of its subnormals at
+    # most. A float's three bf16 parts reach down to bf16's smallest subnormal, 2^-133:
+    # x = hi + mid + lo + r, each part cut towards zero at its eighth bit or at 2^-133,
+    # whichever is more, so |r| < 2^-133, and the weight is 1.
+    assert bool(((got - want).abs() <= fo.half(dtype) * want.abs() + 2.0 ** -133).all())
 
 
 @pytest.mark.parametrize("m", [3, 40, 700])

@@ -18,7 +18,7 @@
 // of two are exact in bf16 (two significant bits, and bf16's exponents and
 // subnormals reach every scale), so they lose nothing on the way in; float
 // activations meet them as three bf16 parts of 8 bits each, whose sum is the
-// float exactly. Float weights take 16x16x4 float MFMAs.
+// float exactly, but for bits below 2^-133, bf16's smallest. Float weights take 16x16x4 float MFMAs.
 #pragma once
 
 #include "common.h"
@@ -71,7 +71,7 @@ template <> struct Piece<float> {
 };
 
 // Floats as three bf16 parts of 8 significant bits each, cut and not rounded: the
-// parts add up to the float. Infinities and NaN sit in the first part alone.
+// parts add up to the float (bits below 2^-133 are cut off). Infinities and NaN sit in the first part alone.
 __device__ __forceinline__ void split3(const Piece<float>& x, u32x4_t& hi, u32x4_t& mid, u32x4_t& lo) {
   constexpr unsigned UPPER = 0x07060302u;                    // the upper halves of two words
 #pragma unroll

@@ -81,10 +81,15 @@ class _Tiles:
         wc = dense(w)
         tiles = -(-n // 16) * -(-k // 128)
         self.data = torch.empty(mats * tiles * 2048, dtype=w.dtype, device=w.device)
-        self.codes_ptr, self.scales_ptr = self.data.data_ptr(), None
         with on_device(w.device):
             native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), self.codes_ptr,
                         stream_of(w.device))
+
+    scales_ptr = None
+
+    @property
+    def codes_ptr(self) -> int:
+        return self.data.data_ptr()
 
 
 class MoeWeights:
@@ -126,13 +131,24 @@ class MoeWeights:
                 self.shared_router = dense(shared_router.detach().reshape(-1))
         elif shared_router is not None:
             raise ValueError("shared_router without shared experts")
+        self._bind()
+
+    def _bind(self) -> None:
+        """The weights as the C ABI takes them (qm_moe_weights)."""
         mats = (self.gate, self.up, self.down, self.s_gate, self.s_up, self.s_down)
         p = [None if t is None else t.codes_ptr for t in mats]
         s = [None if t is None else t.scales_ptr for t in mats]
-        # the weights as the C ABI takes them (qm_moe_weights)
         self.ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
                                          native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
         self._ptrs_ref = ctypes.byref(self.ptrs)
+
+    # a copied or loaded layer has memory of its own
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("ptrs", "_ptrs_ref")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     def _take(self, mats: int, parts, what: str) -> list:
         out = []

@@ -85,8 +85,15 @@ class Mx4Weight:
         self.data, self.shape = data, torch.Size(shape)
         # the codes are 16 of 17 bytes, the scales behind them
         self.code_bytes = data.numel() // 17 * 16
-        self.codes_ptr = data.data_ptr()
-        self.scales_ptr = self.codes_ptr + self.code_bytes
+
+    # (read from the tensor each time: a copied or loaded weight has memory of its own)
+    @property
+    def codes_ptr(self) -> int:
+        return self.data.data_ptr()
+
+    @property
+    def scales_ptr(self) -> int:
+        return self.data.data_ptr() + self.code_bytes
 
     @property
     def codes(self) -> torch.Tensor:
