@@ -128,7 +128,8 @@ def test_linear_keeps_bad_values_to_their_rows(gpu, dtype, m):
 
 # One size for each tiling that many rows can take (the workgroups that a tile
 # leaves decide), at the smallest k that still ends inside a tile of 128.
-TILINGS = [(40, 300), (60, 1300), (40, 4090), (60, 4090), (100, 4090), (170, 4090), (300, 4090), (600, 4090), (1030, 4090), (2000, 1000)]
+TILINGS = [(40, 300), (60, 1300), (40, 4090), (60, 4090), (100, 4090), (170, 4090), (300, 4090), (600, 4090),
+           (700, 4090), (1030, 4090), (1600, 4090), (2000, 1000)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

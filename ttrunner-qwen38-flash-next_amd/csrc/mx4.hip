@@ -249,11 +249,11 @@ int launch_rows(const Mx4LinearArgs<T>& A, hipStream_t stream) {
 // Many activation rows: a workgroup per 16 TN WN weight rows x 16 TM WM
 // activation rows (wgemm.h), the activation rows' tiles of one range of weights
 // side by side on an XCD.
-template <typename T, int TN, int TM, int WN, int WM, int S>
-__global__ __launch_bounds__(64 * WN * WM, 2) void mx4_gemm_kernel(Mx4LinearArgs<T> A) {
-  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S>;
+template <typename T, int TN, int TM, int WN, int WM, int S, int KS>
+__global__ __launch_bounds__(64 * WN * WM * KS, 2) void mx4_gemm_kernel(Mx4LinearArgs<T> A) {
+  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S, false, KS>;
   extern __shared__ __attribute__((aligned(16))) char s_buf[];
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % (WN * WM);
   const int mt = (A.m + G::BM - 1) / G::BM;
   const int item = xcd_run(blockIdx.x, gridDim.x);
   const int m0 = item % mt * G::BM, t0 = item / mt * WN * TN;
@@ -265,6 +265,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void mx4_gemm_kernel(Mx4LinearArgs
   f32x4_t acc[TN][TM];
   clear(acc);
   G::run(acc, s_buf, src, A.k, A.m - m0);
+  if (!G::join(acc, s_buf)) return;
 #pragma unroll
   for (int t = 0; t < TN; ++t)
 #pragma unroll
@@ -272,14 +273,15 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void mx4_gemm_kernel(Mx4LinearArgs
       store4(A, m0 + (wid % WM) * 16 * TM + 16 * u + (lane & 15), (t0 + wid / WM * TN + t) * 16 + 4 * (lane >> 4), acc[t][u]);
 }
 
-template <typename T, int TN, int TM, int WN, int WM, int S>
+template <typename T, int TN, int TM, int WN, int WM, int S, int KS = 1>
 int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
-  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S>;
+  using G = SpanGemm<WMx4, T, TN, TM, WN, WM, S, false, KS>;
+  constexpr int NT = 64 * WN * WM * KS;
   const long nb = (long)((A.rt + TN * WN - 1) / (TN * WN)) * ((A.m + G::BM - 1) / G::BM);
-  if (nb > 0x7fffffffL / (64 * WN * WM)) return qm_fail(QM_ERR_UNSUPPORTED, "qm_mx4_linear: too many tiles for one launch");
-  const int rc = qm_allow_lds(reinterpret_cast<const void*>(mx4_gemm_kernel<T, TN, TM, WN, WM, S>), G::LDS_BYTES);
+  if (nb > 0x7fffffffL / NT) return qm_fail(QM_ERR_UNSUPPORTED, "qm_mx4_linear: too many tiles for one launch");
+  const int rc = qm_allow_lds(reinterpret_cast<const void*>(mx4_gemm_kernel<T, TN, TM, WN, WM, S, KS>), G::LDS_BYTES);
   if (rc) return rc;
-  hipLaunchKernelGGL((mx4_gemm_kernel<T, TN, TM, WN, WM, S>), dim3((unsigned)nb), dim3(64 * WN * WM), G::LDS_BYTES, stream, A);
+  hipLaunchKernelGGL((mx4_gemm_kernel<T, TN, TM, WN, WM, S, KS>), dim3((unsigned)nb), dim3(NT), G::LDS_BYTES, stream, A);
   QM_CHECK_LAUNCH();
   return QM_OK;
 }
@@ -295,24 +297,26 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
 //     every workgroup, so as many tiles as leave one a CU share them, up to eight
 //     (12352 x 2048, 1 row: 1, 2, 4, 8 tiles 12.5 / 8.7 / 7.6 / 10; 32 rows 22 / 16 /
 //     12.0 / 11.5).
-//   bf16, more than 640 of them with four tiles each   the largest of the tiles of
-//     wgemm.h that makes 256 workgroups, else the smallest. 12352 x 2048, few-row
-//     kernel / 128 x 16 / 128 x 32 / 256 x 32 / 256 x 64: 48 rows (579) 10.5 / 10.6 /
-//     12.0 / 13.8 / 19.6, 64 rows (772) 12.7 / 10.4 / 11.9 / 14.1 / 20.5, 128 rows
-//     20.1 / 17.9 / 14.2 / 14.5 / 20.6, 200 rows 28.9 / 21.1 / 18.2 / 20.2 / 21.4; at
-//     2048 x 4096, whose k is longer, the few-row kernel leads up to 512 rows (1024:
-//     17.2 / 18.5)
+//   bf16, more than 512 of them with four tiles each   wgemm.h, its tile by how many
+//     workgroups it makes: 128 x 32 with k over four groups of waves up to one a CU,
+//     over two up to 640; then 256 x 32 up to 768, then 256 x 64. Few-row kernel /
+//     four groups / two / 256 x 32 / 256 x 64, and the number of 128 x 32 tiles: 12352
+//     x 2048: 32 rows (97) 8.4 / 9.2 / 9.9 / 13.7 / 18.1, 48 rows (194) 10.5 / 9.4 /
+//     9.9 / 13.4 / 19.6, 128 rows (388) 20.1 / 16.7 / 13.0 / 14.5 / 20.6, 256 rows
+//     (776) - / 30.5 / 22.9 / 20.0 / 21.2, 512 rows (1552) - / 52 / 40 / 37 / 33.5; 9856
+//     x 2048: 400 rows (1001) 39 / 31 / 23.7 / 21.1 / 29.7; 2048 x 4096: 256 rows (128)
+//     10.4 / 13.4 / 15.4 / 23.0 / 35, 400 rows (208) 16.6 / 13.6 / 15.3 / 19.7 / 35
 //   float   256 x 32 tiles from 512 workgroups on (2000 rows of 9856 x 2048: 283
 //     against 328; 256 of 12352 x 2048, 392 of them: 60 against 63)
 template <typename T>
 int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   auto groups = [&A](int bn, int bm) { return (long)((A.rt * 16 + bn - 1) / bn) * ((A.m + bm - 1) / bm); };
   if constexpr (sizeof(T) == 2) {
-    if (groups(64, 16) > 640) {
-      if (groups(256, 64) >= 256) return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
-      if (groups(256, 32) >= 256) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
-      if (groups(128, 32) >= 256) return launch_gemm<T, 2, 2, 4, 1, 3>(A, stream);
-      return launch_gemm<T, 2, 1, 4, 1, 4>(A, stream);
+    if (groups(64, 16) > 512) {
+      if (groups(128, 32) <= 256) return launch_gemm<T, 2, 2, 4, 1, 2, 4>(A, stream);
+      if (groups(128, 32) <= 640) return launch_gemm<T, 2, 2, 4, 1, 2, 2>(A, stream);
+      if (groups(256, 32) <= 768) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
+      return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
     }
     if (groups(16, 16) <= 256) return launch_rows<T, 1, 16>(A, stream);
     if (groups(32, 16) <= 256) return launch_rows<T, 2, 16>(A, stream);

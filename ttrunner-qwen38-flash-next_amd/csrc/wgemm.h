@@ -19,7 +19,7 @@ __device__ __forceinline__ int xcd_run(int bid, int n) {
   return x * q + min(x, r) + bid / 8;
 }
 
-template <typename WF, typename T, int TN, int TM, int WN, int WM, int S, bool STREAM = false>
+template <typename WF, typename T, int TN, int TM, int WN, int WM, int S, bool STREAM = false, int KS = 1>
 struct SpanGemm {
   using F = Fmt<WF, T>;
   static constexpr int NW = WN * WM;
@@ -30,8 +30,9 @@ struct SpanGemm {
   static constexpr int WL = TN * WN * F::SPAN_B / 1024 / NW;   // weight loads
   static constexpr int W_LOADS = WL + (F::SCALED ? 1 : 0);
   static constexpr int X_B = BM * ROW_B, W_B = TN * WN * F::SPAN_B, S_B = F::SCALED ? NW * 256 : 0;
-  static constexpr int BUF = X_B + W_B + S_B, LDS_BYTES = S * BUF;
+  static constexpr int BUF = X_B + W_B + S_B, LDS_BYTES = KS * S * BUF;
   static_assert(XL * RPL * NW == BM && WL * 1024 * NW == W_B && TN <= 4 && XL > 0 && WL > 0, "loads of a wave");
+  static_assert((KS - 1) * NW * TN * TM * 1024 <= LDS_BYTES, "the groups' sums take the ring's place");
 
   // where this lane's loads come from: activation rows (clamped into the matrix),
   // pieces of weights, and the scales of the wave's own row tiles
@@ -78,17 +79,20 @@ struct SpanGemm {
     if constexpr (F::SCALED) lds_load4(src.s + (long)j * 64, buf + X_B + W_B + wid * 256);
   }
   __device__ __forceinline__ static void run(f32x4_t (&acc)[TN][TM], char* lds, const Src& src, int k, int rows) {
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wid = KS > 1 ? wave % NW : wave, part = KS > 1 ? wave / NW : 0;
+    if constexpr (KS > 1) lds += part * (S * BUF);
     const int g4 = lane >> 4, row0 = (wid % WM) * 16 * TM + (lane & 15), wn = wid / WM;
-    const int spans = (k + F::SPAN - 1) / F::SPAN;
+    // of this group, and of the first, which has as many as any
+    const int all = (k + F::SPAN - 1) / F::SPAN, spans = (all - part + KS - 1) / KS, most = (all + KS - 1) / KS;
 #pragma unroll
     for (int j = 0; j < S - 1; ++j)
-      if (j < spans) fetch(lds + j * BUF, src, k, rows, j, wid, lane);
-    for (int j0 = 0; j0 < spans; j0 += S) {
+      if (j < spans) fetch(lds + j * BUF, src, k, rows, j * KS + part, wid, lane);
+    for (int j0 = 0; j0 < most; j0 += S) {
 #pragma unroll
       for (int b = 0; b < S; ++b) {
         const int j = j0 + b;
-        if (j >= spans) break;
+        if (j >= most) break;
         // this wave's part of span j is in LDS when at most the S - 2 later
         // spans' loads are outstanding (loads return in order; those of
         // activations do not count, a wave whose rows lie past the last makes
@@ -97,14 +101,15 @@ struct SpanGemm {
           wave_loads_barrier<(S - 2) * W_LOADS>();
         else
           wave_loads_barrier<0>();
-        if (j + S - 1 < spans) fetch(lds + (b + S - 1) % S * BUF, src, k, rows, j + S - 1, wid, lane);
+        if (j + S - 1 < spans) fetch(lds + (b + S - 1) % S * BUF, src, k, rows, (j + S - 1) * KS + part, wid, lane);
+        if (KS > 1 && j >= spans) continue;
         const char* buf = lds + b * BUF;
         typename F::W w[TN];
 #pragma unroll
         for (int t = 0; t < TN; ++t)
           F::span_w(w[t], buf + X_B + (wn * TN + t) * F::SPAN_B, buf + X_B + W_B + wid * 256 + t * 64, lane);
-        f32x4_t part[TN][TM];
-        if constexpr (sizeof(T) == 4) clear(part);
+        f32x4_t sum[TN][TM];
+        if constexpr (sizeof(T) == 4) clear(sum);
         // a piece's activations are read while the one before is multiplied
         Piece<T> x[2][TM];
 #pragma unroll
@@ -116,16 +121,40 @@ struct SpanGemm {
             for (int u = 0; u < TM; ++u) x[(s + 1) & 1][u] = lds_piece<T>(buf + (row0 + 16 * u) * ROW_B, F::unit(g4, s + 1), swizzle(row0));
           }
           // float sums in two levels: a span, then the spans
-          if constexpr (sizeof(T) == 4) F::step(part, w, s, x[s & 1]);
+          if constexpr (sizeof(T) == 4) F::step(sum, w, s, x[s & 1]);
           else F::step(acc, w, s, x[s & 1]);
         }
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
           for (int t = 0; t < TN; ++t)
 #pragma unroll
-            for (int u = 0; u < TM; ++u) acc[t][u] += part[t][u];
+            for (int u = 0; u < TM; ++u) acc[t][u] += sum[t][u];
         }
       }
     }
+  }
+  // The groups' sums, in their order, in the first group's waves; false in the others,
+  // which have nothing left to do.
+  __device__ __forceinline__ static bool join(f32x4_t (&acc)[TN][TM], char* lds) {
+    if constexpr (KS > 1) {
+      const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      f32x4_t* s = reinterpret_cast<f32x4_t*>(lds) + lane;
+      __syncthreads();
+      if (wave >= NW) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+          for (int u = 0; u < TM; ++u) s[(((wave - NW) * TN + t) * TM + u) * 64] = acc[t][u];
+      }
+      __syncthreads();
+      if (wave >= NW) return false;
+#pragma unroll
+      for (int p = 0; p < KS - 1; ++p)
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+          for (int u = 0; u < TM; ++u) acc[t][u] += s[(((p * NW + wave) * TN + t) * TM + u) * 64];
+    }
+    return true;
   }
 };
