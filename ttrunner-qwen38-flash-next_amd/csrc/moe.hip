@@ -63,10 +63,10 @@ __device__ __forceinline__ WMat expert_mat(const WMat& m, int e, long tiles, int
 // does and leaves the table of slots.
 //
 // What bounds it is the weights' way from memory. 8 of 128 experts of 2048 x 512 and
-// a shared one: one token, bf16, 57 MB: logits 3.0 us, up 10 to 11.5 (3 of them the
-// ranking), down 5.8; 9 tokens, 4-bit, 107 MB: 4.1, table 5.8, up 15 (4.7 TB/s), down
-// 11. Against the many-token kernels: 8 tokens, 4-bit, 35 for 40 us, 16 tokens 47 and
-// 47, bf16 100 for 110.
+// a shared one: one token, bf16, 57 MB: logits 3.1 us, up 10 to 11.6 (2 of them the
+// ranking), down 6; 9 tokens, 4-bit, 107 MB: 4.1, table 4.6, up 15 (4.7 TB/s), down
+// 11.5. Against the many-token kernels: 8 tokens, 4-bit, 34 for 39 us, 16 tokens 46 and
+// 46, bf16 98 for 108.
 // ---------------------------------------------------------------------------
 constexpr int FEW = 16;
 constexpr int FEW_UP_NW = 8, FEW_DOWN_NW = 16;
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
 // Many tokens: routing, the experts' lists of pairs, the up products, the down
 // products of every pair, and their sum per token.
 //
-// 2000 tokens, 8 of 64 experts of 2048 x 768 and a shared one, bf16: routing 33 us, up
+// 2000 tokens, 8 of 64 experts of 2048 x 768 and a shared one, bf16: routing 30 us, up
 // 163, down 124, sum 25. The up products read 400 MB of weights and do 113 GFLOP (a
 // quarter more with the experts' last tiles filled up): 620 MB from behind the L2 at
 // 3.9 TB/s and 870 TFLOP/s at once, neither alone at its limit. 128 tokens, 4-bit, 8 of

@@ -22,8 +22,8 @@ namespace {
 
 // Products of a call (rows x columns x hidden) up to which every logit is summed in
 // double. Logits and choice of 128 experts over 2048, us, so / by matrix cores: bf16
-// 256 rows (7e7) 18 / 24, 460 rows (1.2e8) 26 / 25, 1000 rows 46 / 26; float 1024
-// rows (2.7e8) 53 / 82, 1500 rows 74 / 84, 2048 rows (5.4e8) 98 / 83.
+// 256 rows (7e7) 17 / 22, 360 rows 21 / 23, 460 rows (1.2e8) 25 / 22, 1000 rows 44 /
+// 23; float 1024 rows (2.7e8) 53 / 80, 1500 rows 73 / 82, 2048 rows (5.4e8) 98 / 81.
 template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 4.5e8;
 // Choices of an expert, on average, up to which the choosing waves file them by
 // atomics (they serialise: 8 each +2.4 us, 16 +4.2, 32 +7.2, 250 +31); beyond, a
@@ -455,9 +455,9 @@ __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P,
     P.weights[(long)t * P.ld_w + P.top_k + lane] = A.cols > A.experts ? sigmoid_f((float)l[A.experts]) : 1.f;
 }
 
-// One wave per token: a chain of a load, top_k selections and, for one token in ten
-// of the many-row logits, another load and two sums in double (4001 tokens over 256
-// experts 17.7 us, one over 128 4.5)
+// One wave per token: a chain of a load, a search and a ranking (moe_topk.h) and, for
+// one token in ten of the many-row logits, another load and two sums in double (4001
+// tokens over 256 experts 14.3 us, one over 128 3.0)
 template <typename T, int PER>
 __global__ __launch_bounds__(256) void moe_topk_kernel(QmLogits<T> A, TopArgs P) {
   const int lane = threadIdx.x & 63;
