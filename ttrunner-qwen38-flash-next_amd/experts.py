@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import native
-from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, on_device, stream_of
+from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, launch
 
 MAX_EXPERTS, MAX_TOP_K, MAX_SHARED = 1024, 32, 32
 
@@ -60,15 +60,12 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool
     weights = torch.empty(lead + (top_k,), dtype=torch.float32, device=device)
     m = lead.numel()
     if m:
-        lib = native.load()
         xr, ldx = activation_rows(x)
         rc = dense(router)
-        nbytes = lib.qm_moe_route_workspace(m, experts)
+        nbytes = native.load().qm_moe_route_workspace(m, experts)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        with on_device(device):
-            native.check("qm_moe_route", lib.qm_moe_route(
-                act, m, hidden, experts, top_k, 1 if normalize else 0, xr.data_ptr(), ldx, rc.data_ptr(), ids.data_ptr(),
-                weights.data_ptr(), ws.data_ptr(), nbytes, stream_of(device)))
+        launch("qm_moe_route", device, act, m, hidden, experts, top_k, 1 if normalize else 0, xr.data_ptr(), ldx,
+               rc.data_ptr(), ids.data_ptr(), weights.data_ptr(), ws.data_ptr(), nbytes)
     return ids, weights
 
 
@@ -81,9 +78,7 @@ class _Tiles:
         wc = dense(w)
         tiles = -(-n // 16) * -(-k // 128)
         self.data = torch.empty(mats * tiles * 2048, dtype=w.dtype, device=w.device)
-        with on_device(w.device):
-            native.call("qm_tile_weight", native.act_code(w.dtype), mats, n, k, native.ptr(wc), self.codes_ptr,
-                        stream_of(w.device))
+        launch("qm_tile_weight", w.device, native.act_code(w.dtype), mats, n, k, wc.data_ptr(), self.codes_ptr)
 
     scales_ptr = None
 
@@ -141,10 +136,11 @@ class MoeWeights:
         self.ptrs = native.MoeWeightPtrs(self.router.data_ptr(), p[0], p[1], p[2], s[0], s[1], s[2],
                                          native.ptr(self.shared_router), p[3], p[4], p[5], s[3], s[4], s[5])
         self._ptrs_ref = ctypes.byref(self.ptrs)
+        self._calls = {}
 
     # a copied or loaded layer has memory of its own
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k not in ("ptrs", "_ptrs_ref")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("ptrs", "_ptrs_ref", "_calls")}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -183,6 +179,17 @@ class MoeWeights:
                               int(self.normalize), native.act_code(self.dtype),
                               native.QM_W_MX4 if self.is_mx4 else native.QM_W_ACT)
 
+    def _call(self, rows: int):
+        """(geometry, bytes of workspace) of a call of ``rows`` tokens, kept for the
+        next of as many."""
+        hit = self._calls.get(rows)
+        if hit is None:
+            if len(self._calls) >= 256:
+                self._calls.clear()
+            g = ctypes.byref(self.geom(rows))
+            hit = self._calls[rows] = (g, max(native.load().qm_moe_workspace(g), 1))
+        return hit
+
 
 def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
     """The layer's output for x [..., hidden] (the weights' type), in x's shape:
@@ -193,12 +200,8 @@ def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
     out = torch.empty(x.shape, dtype=x.dtype, device=device)
     m = x.shape[:-1].numel()
     if m:
-        lib = native.load()
         xr, ldx = activation_rows(x)
-        g = ctypes.byref(weights.geom(m))
-        nbytes = lib.qm_moe_workspace(g)
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-        with on_device(device):
-            native.check("qm_moe", lib.qm_moe(g, weights._ptrs_ref, xr.data_ptr(), ldx, out.data_ptr(), ws.data_ptr(),
-                                              nbytes, stream_of(device)))
+        g, nbytes = weights._call(m)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        launch("qm_moe", device, g, weights._ptrs_ref, xr.data_ptr(), ldx, out.data_ptr(), ws.data_ptr(), nbytes)
     return out

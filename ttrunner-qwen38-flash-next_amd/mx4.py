@@ -16,7 +16,6 @@ inputs that require a gradient are refused while gradients are recorded.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -27,19 +26,20 @@ BLOCK = 32
 TILE_ROWS, TILE_K = 16, 128
 
 
-_HERE = contextlib.nullcontext()
 _ACT = {torch.float32: native.QM_ACT_F32, torch.bfloat16: native.QM_ACT_BF16}
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def on_device(device):
-    """A context in which ``device`` is the current one (launches go there)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def stream_of(device) -> int:
-    """The handle of the device's current stream."""
-    return _raw_stream(device.index)
+def launch(name: str, device, *args) -> None:
+    """The entry point ``name`` on ``args`` and the current stream of ``device``."""
+    fn, index = getattr(native.load(), name), device.index
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):                             # kernels go to the current device
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        native.check(name, rc)
 
 
 def check_input(t: torch.Tensor, what: str) -> int:
@@ -140,9 +140,8 @@ class Mx4Weight:
                              f"got {tuple(scales.shape)} on {scales.device}")
         w = cls._empty(shape, codes.device)
         pc, ps = dense(codes), scales.contiguous()
-        with on_device(codes.device):
-            native.call("qm_mx4_layout", 1, w.mats, shape[-2], shape[-1], w.codes_ptr, w.scales_ptr,
-                        native.ptr(pc), native.ptr(ps), stream_of(codes.device))
+        launch("qm_mx4_layout", codes.device, 1, w.mats, shape[-2], shape[-1], w.codes_ptr, w.scales_ptr, pc.data_ptr(),
+               ps.data_ptr())
         return w
 
     def plain(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -150,9 +149,8 @@ class Mx4Weight:
         lead, n, k = self.shape[:-2], self.shape[-2], self.shape[-1]
         codes = torch.empty(*lead, n, k // 2, dtype=torch.uint8, device=self.device)
         scales = torch.empty(*lead, n, k // BLOCK, dtype=torch.uint8, device=self.device)
-        with on_device(self.device):
-            native.call("qm_mx4_layout", 0, self.mats, n, k, self.codes_ptr, self.scales_ptr,
-                        native.ptr(codes), native.ptr(scales), stream_of(self.device))
+        launch("qm_mx4_layout", self.device, 0, self.mats, n, k, self.codes_ptr, self.scales_ptr, codes.data_ptr(),
+               scales.data_ptr())
         return codes, scales
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -161,9 +159,8 @@ class Mx4Weight:
         shape, device = self.shape, self.data.device
         act = native.act_code(dtype)
         out = torch.empty(shape, dtype=dtype, device=device)
-        with on_device(device):
-            native.check("qm_mx4_dequantize", native.load().qm_mx4_dequantize(
-                act, self.mats, shape[-2], shape[-1], self.codes_ptr, self.scales_ptr, out.data_ptr(), stream_of(device)))
+        launch("qm_mx4_dequantize", device, act, self.mats, shape[-2], shape[-1], self.codes_ptr, self.scales_ptr,
+               out.data_ptr())
         return out
 
 
@@ -176,9 +173,7 @@ def mx4_quantize(w: torch.Tensor) -> Mx4Weight:
     shape, device = w.shape, w.device
     out = Mx4Weight._empty(shape, device)
     wc = dense(w)
-    with on_device(device):
-        native.check("qm_mx4_quantize", native.load().qm_mx4_quantize(
-            act, out.mats, shape[-2], shape[-1], wc.data_ptr(), out.codes_ptr, out.scales_ptr, stream_of(device)))
+    launch("qm_mx4_quantize", device, act, out.mats, shape[-2], shape[-1], wc.data_ptr(), out.codes_ptr, out.scales_ptr)
     return out
 
 
@@ -196,7 +191,7 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Weight, sections=None):
     if not lead or lead[-1] != k:
         raise ValueError(f"x must be [..., {k}], got {tuple(lead)}")
     device = x.device
-    if device != weight.device:
+    if device != weight.data.device:
         raise ValueError(f"x is on {device}, the weight on {weight.device}")
     lead = lead[:-1]
     m = lead.numel()
@@ -208,10 +203,12 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Weight, sections=None):
     outs = [torch.empty(lead + (r,), dtype=x.dtype, device=device) for r in rows]
     if m:
         xr, ldx = activation_rows(x)
-        seg_rows = (ctypes.c_int * len(rows))(*rows)
-        seg_out = (ctypes.c_void_p * len(rows))(*[o.data_ptr() for o in outs])
-        with on_device(device):
-            native.check("qm_mx4_linear", native.load().qm_mx4_linear(
-                act, m, n, k, weight.codes_ptr, weight.scales_ptr, xr.data_ptr(), ldx, len(rows), seg_rows,
-                seg_out, stream_of(device)))
+        if sections is None:
+            seg_rows, seg_out = ctypes.byref(ctypes.c_int(n)), ctypes.byref(ctypes.c_void_p(outs[0].data_ptr()))
+        else:
+            seg_rows = (ctypes.c_int * len(rows))(*rows)
+            seg_out = (ctypes.c_void_p * len(rows))(*[o.data_ptr() for o in outs])
+        codes = weight.data.data_ptr()
+        launch("qm_mx4_linear", device, act, m, n, k, codes, codes + weight.code_bytes, xr.data_ptr(), ldx, len(rows),
+               seg_rows, seg_out)
     return outs[0] if sections is None else outs
