@@ -82,7 +82,8 @@ class Mx4Weight:
     stand for."""
 
     def __init__(self, data: torch.Tensor, shape):
-        self.data, self.shape = data, torch.Size(shape)
+        self.data, self.shape = data, shape if type(shape) is torch.Size else torch.Size(shape)
+        self.mats = 1 if len(shape) == 2 else self.shape[:-2].numel()
         # the codes are 16 of 17 bytes, the scales behind them
         self.code_bytes = data.numel() // 17 * 16
 
@@ -107,11 +108,6 @@ class Mx4Weight:
     def device(self):
         return self.data.device
 
-    @property
-    def mats(self) -> int:
-        """Matrices in it (the product of the leading dimensions)."""
-        return self.shape[:-2].numel()
-
     @staticmethod
     def _check_shape(shape) -> None:
         if len(shape) < 2 or 0 in shape:
@@ -121,9 +117,11 @@ class Mx4Weight:
 
     @classmethod
     def _empty(cls, shape, device) -> "Mx4Weight":
-        shape = torch.Size(shape)
         cls._check_shape(shape)
-        tiles = shape[:-2].numel() * -(-shape[-2] // TILE_ROWS) * -(-shape[-1] // TILE_K)
+        n, k = shape[-2:]
+        tiles = -(-n // TILE_ROWS) * -(-k // TILE_K)
+        if len(shape) > 2:
+            tiles *= shape[:-2].numel()
         return cls(torch.empty(tiles * (TILE_ROWS * TILE_K // 32 * 17), dtype=torch.uint8, device=device), shape)
 
     @classmethod
@@ -133,7 +131,7 @@ class Mx4Weight:
         and scale bytes uint8 [..., n, k / 32] (2^(byte - 127), 255 NaN)."""
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda:
             raise ValueError("codes and scales must be uint8 tensors on the GPU")
-        shape = codes.shape[:-1] + (2 * codes.shape[-1],)
+        shape = torch.Size(codes.shape[:-1] + (2 * codes.shape[-1],))
         cls._check_shape(shape)
         if scales.shape != codes.shape[:-1] + (shape[-1] // BLOCK,) or scales.device != codes.device:
             raise ValueError(f"scales must be {tuple(codes.shape[:-1]) + (shape[-1] // BLOCK,)} on {codes.device}, "
