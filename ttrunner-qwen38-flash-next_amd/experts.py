@@ -13,6 +13,7 @@ the tensors' device. Nothing here is differentiable.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -20,6 +21,11 @@ from . import native
 from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, launch
 
 MAX_EXPERTS, MAX_TOP_K, MAX_SHARED = 1024, 32, 32
+
+
+@functools.lru_cache(256)
+def _route_bytes(rows: int, experts: int) -> int:
+    return native.load().qm_moe_route_workspace(rows, experts)
 
 
 def _check_router(x: torch.Tensor, router: torch.Tensor, top_k: int) -> None:
@@ -55,14 +61,14 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool
     _check_router_shape(router)
     _check_router(x, router, top_k)
     experts, hidden = router.shape
-    lead, device = x.shape[:-1], x.device
-    ids = torch.empty(lead + (top_k,), dtype=torch.int32, device=device)
-    weights = torch.empty(lead + (top_k,), dtype=torch.float32, device=device)
-    m = lead.numel()
+    shape, device = x.shape[:-1] + (top_k,), x.device
+    ids = torch.empty(shape, dtype=torch.int32, device=device)
+    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    m = x.numel() // hidden
     if m:
         xr, ldx = activation_rows(x)
         rc = dense(router)
-        nbytes = native.load().qm_moe_route_workspace(m, experts)
+        nbytes = _route_bytes(m, experts)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         launch("qm_moe_route", device, act, m, hidden, experts, top_k, 1 if normalize else 0, xr.data_ptr(), ldx,
                rc.data_ptr(), ids.data_ptr(), weights.data_ptr(), ws.data_ptr(), nbytes)
@@ -198,7 +204,7 @@ def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
     _check_router(x, weights.router, weights.top_k)
     device = x.device
     out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    m = x.shape[:-1].numel()
+    m = x.numel() // weights.hidden
     if m:
         xr, ldx = activation_rows(x)
         g, nbytes = weights._call(m)
