@@ -204,10 +204,12 @@ __global__ __launch_bounds__(64 * FEW_UP_NW) void moe_few_up_kernel(FewArgs<T> A
       if (slot == 0) clear_down(A, threadIdx.x, 16);
     }
   } else {
-    if (slot >= *A.n_slots) return;
+    // (one round trip: what stands behind the last slot is read but not used)
+    const int n = *A.n_slots;
     e = A.slot_expert[slot];
     pair = A.slot_pair[slot * 16 + r16];
     weight = A.slot_w[slot * 16 + r16];
+    if (slot >= n) return;
   }
   const WMat gate = expert_mat(e < 0 ? M.s_gate : M.gate, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
   const WMat up = expert_mat(e < 0 ? M.s_up : M.up, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
@@ -266,15 +268,16 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
   const int kt = wt_k_tiles(M.inter), rt = wt_row_tiles(M.hidden);
   const int units = *A.n_slots * kt, stride = NW * A.split, first = NW * blockIdx.y + wid;
   f32x4_t total = {0.f, 0.f, 0.f, 0.f};
-  // a batch's slots are looked up while the one before is multiplied
+  // a batch's slots are looked up while the one before is multiplied, the first
+  // while their number is on its way (what stands behind the last is not used)
+  const int most = M.shared + min(M.rows * M.top_k, M.experts);
   int expert[U], pair[U], at[U];
   int slot = first / kt, ks = first % kt;                    // of the next unit to look up
   const int slot_step = stride / kt, ks_step = stride % kt;
-  const int last = units / kt - 1;
   auto look_up = [&]() {
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int s = min(slot, last);
+      const int s = min(slot, most - 1);
       expert[p] = A.slot_expert[s];
       pair[p] = A.slot_pair[s * 16 + r16];
       at[p] = ks;
@@ -290,12 +293,13 @@ __global__ __launch_bounds__(64 * FEW_DOWN_NW) void moe_few_down_kernel(FewArgs<
     bool mine[U];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int e = expert[p];
+      const bool in = u0 + p * stride < units;
+      const int e = in ? expert[p] : 0;
       const WMat down = expert_mat(e < 0 ? M.s_down : M.down, e < 0 ? -1 - e : e, (long)rt * kt, F::TILE);
       w[p][0] = F::load_w(down, (long)blockIdx.x * kt + at[p], lane);
       // (columns that did not choose the expert load nothing: most of them)
-      mine[p] = pair[p] >= 0;
-      x[p][0].load(M.h + (long)max(pair[p], 0) * M.inter, at[p], mine[p] ? M.inter : 0, g4);
+      mine[p] = in && pair[p] >= 0;
+      x[p][0].load(M.h + (long)(mine[p] ? pair[p] : 0) * M.inter, at[p], mine[p] ? M.inter : 0, g4);
     }
     look_up();
 #pragma unroll
