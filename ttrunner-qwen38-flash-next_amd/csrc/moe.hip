@@ -69,6 +69,8 @@ __device__ __forceinline__ WMat expert_mat(const WMat& m, int e, long tiles, int
 // 46, bf16 98 for 108.
 // ---------------------------------------------------------------------------
 constexpr int FEW = 16;
+// Waves of a workgroup. Down products of 9 tokens, 4-bit: 16 waves with four units in
+// flight each 14.8 us, 8 with eight 16.7 (one workgroup a tile).
 constexpr int FEW_UP_NW = 8, FEW_DOWN_NW = 16;
 
 template <typename T>

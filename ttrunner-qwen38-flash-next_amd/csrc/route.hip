@@ -130,20 +130,20 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
 
 // The same by matrix cores: a workgroup per 64 router rows x 64 tokens (those of the
 // same tokens on one XCD, whose L2 then reads them once), both kinds of rows in LDS
-// (128 k of each at a time, units exchanged as in wgemm.h), a wave per 16 x 32.
-// norms: |R[r]|^2, then |x[t]|^2, the diagonals of products of 16 rows with
+// (two stages of LG_SPANS times 128 k, units exchanged as in wgemm.h), a wave per
+// 16 x 32. norms: |R[r]|^2, then |x[t]|^2, the diagonals of products of 16 rows with
 // themselves, by the first workgroups of a column or a row of tiles. A span takes a
-// workgroup 0.6 to 0.8 us whatever else runs, its loads, its reads of LDS and the
-// steps between them one after the other (bf16, 256 experts over 2048: 4001 rows 17.8
-// us; 64 experts, 2000 rows 15; a tile of 32 x 32 a wave and a quarter of k took as
-// long, a fifth buffer too).
+// workgroup 0.6 us whatever else runs, its loads, its reads of LDS and the steps
+// between them one after the other (bf16, 256 experts over 2048: 4001 rows 16.9 us;
+// 64 experts, 2000 rows 13; with stages of one span, four or five of them, 17.6 and
+// 15; 32 x 32 a wave and a quarter of k 17.5 and 14).
 constexpr int LG_ROWS = 128;
-template <typename T> constexpr int LG_S = sizeof(T) == 2 ? 4 : 2;
+template <typename T> constexpr int LG_SPANS = sizeof(T) == 2 ? 2 : 1;
 
 template <typename T>
 __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, float* norms) {
   constexpr int ROW_B = WT_K * sizeof(T), UNITS = ROW_B / 16, VE = 16 / sizeof(T), RPL = 1024 / ROW_B;
-  constexpr int LOADS = LG_ROWS / RPL / 8, BUF = LG_ROWS * ROW_B, S = LG_S<T>;
+  constexpr int LOADS = LG_ROWS / RPL / 8, BUF = LG_ROWS * ROW_B, SP = LG_SPANS<T>;
   extern __shared__ __attribute__((aligned(16))) char s_buf[];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
@@ -157,19 +157,20 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
     src[i] = row < 64 ? router_row(A, min(e0 + row, A.cols - 1)) : A.x + (long)min(t0 + row - 64, A.rows - 1) * A.ldx;
   }
   auto fetch = [&](int j) {
-    char* buf = s_buf + j % S * BUF;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int row = (wid * LOADS + i) * RPL + lane / UNITS;
-      const int k = j * WT_K + ((lane % UNITS) ^ (row & 15)) * VE;
-      lds_load16(k < A.hidden ? static_cast<const void*>(src[i] + k) : g_zero_unit, buf + (wid * LOADS + i) * 1024);
+    for (int h = 0; h < SP; ++h) {
+      char* buf = s_buf + (j % 2 * SP + h) * BUF;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = (wid * LOADS + i) * RPL + lane / UNITS;
+        const int k = (j * SP + h) * WT_K + ((lane % UNITS) ^ (row & 15)) * VE;
+        lds_load16(k < A.hidden ? static_cast<const void*>(src[i] + k) : g_zero_unit, buf + (wid * LOADS + i) * 1024);
+      }
     }
   };
-  const int spans = wt_k_tiles(A.hidden);
+  const int stages = (wt_k_tiles(A.hidden) + SP - 1) / SP;
   clear_counts(A);
-#pragma unroll
-  for (int j = 0; j < S - 1; ++j)
-    if (j < spans) fetch(j);
+  fetch(0);
   double acc[2][4];
   f32x4_t gram[3];                                           // of the router rows, of the tokens
 #pragma unroll
@@ -178,39 +179,41 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[u][i] = 0.0;
-  for (int j = 0; j < spans; ++j) {
-    if (j + S - 2 < spans) wave_loads_barrier<(S - 2) * LOADS>();
-    else wave_loads_barrier<0>();
-    if (j + S - 1 < spans) fetch(j + S - 1);
-    const char* buf = s_buf + j % S * BUF;
-    Piece<T> a[4], b[4][2];
+  for (int j = 0; j < stages; ++j) {
+    wave_loads_barrier<0>();
+    if (j + 1 < stages) fetch(j + 1);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      a[s] = lds_piece<T>(buf + ((wid >> 1) * 16 + r16) * ROW_B, 4 * s + g4, r16);
+    for (int h = 0; h < SP; ++h) {
+      const char* buf = s_buf + (j % 2 * SP + h) * BUF;
+      Piece<T> a[4], b[4][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[s][h] = lds_piece<T>(buf + (64 + (wid & 1) * 32 + 16 * h + r16) * ROW_B, 4 * s + g4, r16);
-    }
-    __builtin_amdgcn_sched_barrier(0);                       // all reads in flight before the first product
-    f32x4_t part[1][2];
-    clear(part);
+      for (int s = 0; s < 4; ++s) {
+        a[s] = lds_piece<T>(buf + ((wid >> 1) * 16 + r16) * ROW_B, 4 * s + g4, r16);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) part[0][u] = mma_piece(a[s], b[s][u], part[0][u]);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
-    if (w_norm) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) gram[0] = mma_piece(a[s], a[s], gram[0]);
-    }
-    if (x_norm) {
+        for (int u = 0; u < 2; ++u)
+          b[s][u] = lds_piece<T>(buf + (64 + (wid & 1) * 32 + 16 * u + r16) * ROW_B, 4 * s + g4, r16);
+      }
+      __builtin_amdgcn_sched_barrier(0);                     // all reads in flight before the first product
+      f32x4_t part[1][2];
+      clear(part);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) gram[1 + u] = mma_piece(b[s][u], b[s][u], gram[1 + u]);
+        for (int u = 0; u < 2; ++u) part[0][u] = mma_piece(a[s], b[s][u], part[0][u]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
+      if (w_norm) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) gram[0] = mma_piece(a[s], a[s], gram[0]);
+      }
+      if (x_norm) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) gram[1 + u] = mma_piece(b[s][u], b[s][u], gram[1 + u]);
+      }
     }
   }
   // a wave's lane holds rows 4 g4 + i of column r16
@@ -496,7 +499,7 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
     rc = qm_route_logits(A, stream);
   } else {
     P.norms = norms;
-    const size_t lds = (size_t)LG_S<T> * LG_ROWS * WT_K * sizeof(T);
+    const size_t lds = (size_t)2 * LG_SPANS<T> * LG_ROWS * WT_K * sizeof(T);
     rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds);
     if (rc) return rc;
     hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64 * ((A.rows + 63) / 64)), dim3(512), lds, stream, A, norms);
