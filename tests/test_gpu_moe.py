@@ -74,6 +74,25 @@ def test_route_ties_and_bad_values(gpu, t):
     assert bool((ids3[:, 0] == 8).all()) and bool(w3.isnan().all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,e,k", [(1, 50, 6), (5, 100, 8), (1, 300, 32), (20, 700, 3)])
+def test_route_magnitudes_and_many_equal_logits(gpu, dtype, t, e, k):
+    """Logits far below and above float's range, and more equal ones than a wave's lanes."""
+    h = 160
+    x, r = normal(t, t, h, dtype=dtype), normal(e, e, h, dtype=dtype, scale=h ** -0.5)
+    for scale in (2.0 ** -100, 2.0 ** 100):
+        xs, rs = x * scale, r * scale                               # powers of two: the same order
+        ids, w = gpu.moe_route(xs, rs, k)
+        assert torch.equal(ids, fo.route(xs, rs, k)[0]) and torch.equal(ids, fo.route(x, r, k)[0])
+        assert bool((w.sum(-1) - 1).abs().max() < 2.0 ** -20)
+    big = (x.double() @ r.double().t()).argmax(-1)[0].item()
+    r[::2] = r[big]                                                 # half of the experts lead the first token
+    ids, w = gpu.moe_route(x, r, k)
+    assert torch.equal(ids, fo.route(x, r, k)[0])
+    ids, w = gpu.moe_route(torch.zeros_like(x), r, k)
+    assert ids.tolist() == [list(range(k))] * t and torch.equal(w, torch.full_like(w, w[0, 0].item()))
+
+
 def test_route_does_not_depend_on_the_rows_beside(gpu):
     x, r = normal(5, 300, 512, dtype=BF16), normal(6, 96, 512, dtype=BF16, scale=0.05)
     ids, w = gpu.moe_route(x, r, 7)
