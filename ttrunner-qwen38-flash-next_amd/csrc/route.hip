@@ -23,8 +23,8 @@ namespace {
 // Products of a call (rows x columns x hidden) up to which every logit is summed in
 // double. Logits and choice of 128 experts over 2048, us, so / by matrix cores: bf16
 // 256 rows (7e7) 17 / 22, 360 rows 21 / 23, 460 rows (1.2e8) 25 / 22, 1000 rows 44 /
-// 23; float 1024 rows (2.7e8) 53 / 80, 1500 rows 73 / 82, 2048 rows (5.4e8) 98 / 81.
-template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 4.5e8;
+// 23; float 1024 rows (2.7e8) 53 / 70, 1500 rows (3.9e8) 73 / 70, 2048 rows 98 / 70.
+template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 4e8;
 // Choices of an expert, on average, up to which the choosing waves file them by
 // atomics (they serialise: 8 each +2.4 us, 16 +4.2, 32 +7.2, 250 +31); beyond, a
 // launch of its own does (6.0 us and its start, 7.7 at 16000 choices)
@@ -136,7 +136,8 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(QmLogits<T> A) {
 // workgroup 0.6 us whatever else runs, its loads, its reads of LDS and the steps
 // between them one after the other (bf16, 256 experts over 2048: 4001 rows 16.9 us;
 // 64 experts, 2000 rows 13; with stages of one span, four or five of them, 17.6 and
-// 15; 32 x 32 a wave and a quarter of k 17.5 and 14).
+// 15; 32 x 32 a wave and a quarter of k 17.5 and 14). Float products are bound by the
+// matrix cores: 4000 rows over 256 experts 64 us, 76 with the norms in fewer waves.
 constexpr int LG_ROWS = 128;
 template <typename T> constexpr int LG_SPANS = sizeof(T) == 2 ? 2 : 1;
 
@@ -149,7 +150,9 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   const int g4 = lane >> 4, r16 = lane & 15;
   const int et = (A.cols + 63) / 64, item = xcd_run(blockIdx.x, gridDim.x);
   const int e0 = item % et * 64, t0 = item / et * 64;
-  const bool w_norm = item < et && (wid & 1) == 0, x_norm = e0 == 0 && wid < 2;
+  // a group of 16 rows a wave: of the four of router rows waves 0, 2, 5 and 7, of the
+  // tokens' 4, 6, 1 and 3 (each multiplies them anyway)
+  const bool of_router = (((wid >> 2) ^ wid) & 1) == 0, norm = of_router ? item < et : e0 == 0;
   const T* src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -172,9 +175,7 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
   clear_counts(A);
   fetch(0);
   double acc[2][4];
-  f32x4_t gram[3];                                           // of the router rows, of the tokens
-#pragma unroll
-  for (int u = 0; u < 3; ++u) gram[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f32x4_t gram = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -204,28 +205,23 @@ __global__ __launch_bounds__(512) void moe_logits_mma_kernel(QmLogits<T> A, floa
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[u][i] += (double)part[0][u][i];
-      if (w_norm) {
+      if (norm && of_router) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) gram[0] = mma_piece(a[s], a[s], gram[0]);
-      }
-      if (x_norm) {
+        for (int s = 0; s < 4; ++s) gram = mma_piece(a[s], a[s], gram);
+      } else if (norm && (wid & 2)) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 4; ++s) gram = mma_piece(b[s][1], b[s][1], gram);
+      } else if (norm) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) gram[1 + u] = mma_piece(b[s][u], b[s][u], gram[1 + u]);
+        for (int s = 0; s < 4; ++s) gram = mma_piece(b[s][0], b[s][0], gram);
       }
     }
   }
-  // a wave's lane holds rows 4 g4 + i of column r16
-  if ((r16 >> 2) == g4) {
-    auto diagonal = [&](const f32x4_t& g) { return (r16 & 2) ? (r16 & 1) ? g[3] : g[2] : (r16 & 1) ? g[1] : g[0]; };
-    const int r = e0 + (wid >> 1) * 16 + r16;
-    if (w_norm && r < A.cols) norms[r] = diagonal(gram[0]);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = t0 + (wid & 1) * 32 + 16 * u + r16;
-      if (x_norm && t < A.rows) norms[A.cols + t] = diagonal(gram[1 + u]);
-    }
+  // a lane holds rows 4 g4 + i of column r16: the diagonal's element in one of four
+  if (norm && (r16 >> 2) == g4) {
+    const float n = (r16 & 2) ? (r16 & 1) ? gram[3] : gram[2] : (r16 & 1) ? gram[1] : gram[0];
+    const int r = of_router ? e0 + (wid >> 1) * 16 + r16 : t0 + (wid & 1) * 32 + (wid & 2) * 8 + r16;
+    if (r < (of_router ? A.cols : A.rows)) norms[of_router ? r : A.cols + r] = n;
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
