@@ -1,0 +1,58 @@
+"""The experts' and the 4-bit weights' entry points in states that a program around
+them brings about: buffers used again, transforms of autograd, tracing, magnitudes
+beyond float's range, very wide weights, skewed routers."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def normal(seed, *shape, dtype=F32, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def layer_tensors(seed, e, h, i, shared, dtype):
+    """(router, [gate, up, down], shared (gate, up, down), shared_router)"""
+    def mats(s, n):
+        return [normal(s, n, i, h, dtype=dtype, scale=h ** -0.5), normal(s + 1, n, i, h, dtype=dtype, scale=h ** -0.5),
+                normal(s + 2, n, h, i, dtype=dtype, scale=i ** -0.5)]
+    return (normal(seed, e, h, dtype=dtype, scale=h ** -0.5), mats(seed + 1, e), mats(seed + 4, shared),
+            normal(seed + 7, h, dtype=dtype, scale=h ** -0.5))
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("t", [1, 5, 40])
+def test_a_layer_keeps_its_weights_when_their_buffers_are_used_again(gpu, fmt, t):
+    router, mats, shared, shared_router = layer_tensors(1, 8, 96, 64, 1, BF16)
+    lay = gpu.mx4_quantize if fmt == "mx4" else (lambda m: m)
+    w = gpu.MoeWeights(router, *(lay(m) for m in mats), top_k=2, shared=[lay(m) for m in shared], shared_router=shared_router)
+    x = normal(t, t, 96, dtype=BF16)
+    want = gpu.moe(x, w)
+    for buf in (router, shared_router, *mats, *shared):
+        buf.copy_(normal(99, *buf.shape, dtype=BF16))              # the next layer's
+        assert torch.equal(gpu.moe(x, w), want)
+
+
+@pytest.mark.parametrize("fmt", ["act", "mx4"])
+def test_a_model_keeps_a_layers_router_when_the_store_changes(gpu, fmt):
+    """A store whose tensors are on the device already, in the activations' type."""
+    router, (gate, up, down), (sg, su, sd), row = layer_tensors(5, 8, 96, 64, 1, BF16)
+    blk = {"gate_inp": router, "gate_exps": gate, "up_exps": up, "down_exps": down, "gate_shexp": sg[0], "up_shexp": su[0],
+           "down_shexp": sd[0], "gate_inp_shexp": row.view(1, -1)}
+
+    class Store:
+        def get(self, name):
+            return blk[name.split("ffn_")[1].removesuffix(".weight")]
+
+    model = gpu.Qwen4MixModel(gpu.MixConfig(hidden_size=96, num_experts_per_tok=2), Store(), device=DEV, weight_format=fmt)
+    x = normal(2, 1, 7, 96, dtype=BF16)
+    want = model._moe(x, 0)
+    for t in blk.values():
+        t.neg_()
+    assert torch.equal(model._moe(x, 0), want)

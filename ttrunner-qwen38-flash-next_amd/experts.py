@@ -75,6 +75,12 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool
     return ids, weights
 
 
+def _copy(t: torch.Tensor) -> torch.Tensor:
+    """t in memory of its own, as the other weights have it: a loader may read the
+    next layer into the same buffer."""
+    return t.detach().clone(memory_format=torch.contiguous_format)
+
+
 class _Tiles:
     """A weight [mats, n, k] of the activations' type in the kernels' tile order."""
 
@@ -94,7 +100,8 @@ class _Tiles:
 
 
 class MoeWeights:
-    """The weights of a mixture-of-experts layer, laid out once for the kernels.
+    """The weights of a mixture-of-experts layer, copied and laid out once for the
+    kernels (an ``Mx4Weight`` is such a copy already and is kept as it is).
 
     ``router`` [experts, hidden] sets the activations' type; ``gate``, ``up``
     [experts, inter, hidden] and ``down`` [experts, hidden, inter] are tensors of
@@ -105,7 +112,7 @@ class MoeWeights:
 
     def __init__(self, router, gate, up, down, top_k: int, shared=None, shared_router=None, normalize: bool = True):
         _check_router_shape(router)
-        self.router = dense(router.detach())
+        self.router = _copy(router)
         self.experts, self.hidden = router.shape
         self.top_k, self.normalize = int(top_k), bool(normalize)
         if not 1 <= self.top_k <= min(self.experts, MAX_TOP_K):
@@ -129,7 +136,7 @@ class MoeWeights:
                 if shared_router.numel() != self.hidden or shared_router.dtype != router.dtype \
                         or shared_router.device != router.device:
                     raise ValueError(f"shared_router must be [{self.hidden}] in {router.dtype} on {router.device}")
-                self.shared_router = dense(shared_router.detach().reshape(-1))
+                self.shared_router = _copy(shared_router.reshape(-1))
         elif shared_router is not None:
             raise ValueError("shared_router without shared experts")
         self._bind()
