@@ -7,6 +7,9 @@ from __future__ import annotations
 import pytest
 import torch
 
+import ffn_oracle as fo
+from margins import record
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF16, F32 = torch.bfloat16, torch.float32
@@ -56,3 +59,26 @@ def test_a_model_keeps_a_layers_router_when_the_store_changes(gpu, fmt):
     for t in blk.values():
         t.neg_()
     assert torch.equal(model._moe(x, 0), want)
+
+
+@pytest.mark.parametrize("dtype,t,e", [(BF16, 2000, 64), (F32, 2600, 160)])
+def test_shared_gate_beyond_floats_range(gpu, dtype, t, e):
+    """Products of the shared experts' row past float's range that cancel: with many
+    rows (the matrix cores' sums) as with one."""
+    h, i = 1024, 32
+    router, mats, shared, row = layer_tensors(11, e, h, i, 1, dtype)
+    row[0], row[1] = 2.0 ** 120, -2.0 ** 120
+    x = normal(12, t, h, dtype=dtype)
+    x[3] = 0
+    x[3, :2] = 2.0 ** 30                                            # 2^150 - 2^150: the gate is 1/2
+    x[t - 1] = 0
+    x[t - 1, 0] = x[t - 1, 1] = -2.0 ** 10
+    x[7, :2] = 0
+    w = gpu.MoeWeights(router, *mats, top_k=2, shared=shared, shared_router=row)
+    got = gpu.moe(x, w)
+    pick = [0, 3, 7, 8, t - 1]
+    want, bound = fo.moe(x[pick], router.double(), *(m.double() for m in mats), 2, shared=[m.double() for m in shared],
+                         shared_router=row)
+    assert record("bound", fo.within(got[pick], want, bound, dtype), 1.0) <= 1.0
+    for r in pick:
+        assert record("alone", fo.within(gpu.moe(x[r:r + 1], w)[0], want[pick.index(r)], bound[pick.index(r)], dtype), 1.0) <= 1.0

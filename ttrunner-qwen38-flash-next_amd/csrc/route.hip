@@ -243,8 +243,8 @@ struct TopArgs {
   const float* norms;  // null: the logits are sums in double already
 };
 
-// The logits of two experts in double (a close pair, mostly), by the wave: lane c < 2
-// gets expert c's. One round trip for both; the lanes' partial sums meet in the order
+// The logits of two columns in double (a close pair, mostly), by the wave: lane c < 2
+// gets that of e[c]. One round trip for both; the lanes' partial sums meet in the order
 // of their numbers' bits, whichever two are asked for.
 constexpr int EXACT = RT_EXACT;
 template <typename T>
@@ -262,7 +262,7 @@ __device__ __forceinline__ double exact_logits(const QmLogits<T>& A, int t, cons
       const long at = (long)min(u0 + 64 * b, units - 1) * VE;
       xu[b] = *reinterpret_cast<const uint4*>(x + at);
 #pragma unroll
-      for (int c = 0; c < EXACT; ++c) wu[c][b] = *reinterpret_cast<const uint4*>(A.router + (long)e[c] * A.hidden + at);
+      for (int c = 0; c < EXACT; ++c) wu[c][b] = *reinterpret_cast<const uint4*>(router_row(A, e[c]) + at);
     }
 #pragma unroll
     for (int b = 0; b < B; ++b) {
@@ -450,8 +450,20 @@ __device__ __forceinline__ void topk_row(const QmLogits<T>& A, const TopArgs& P,
       P.lists.lists[(long)id * A.rows + at] = t * P.lists.ppt + lane;
     }
   }
-  if (lane < P.shared)
-    P.weights[(long)t * P.ld_w + P.top_k + lane] = A.cols > A.experts ? sigmoid_f((float)l[A.experts]) : 1.f;
+  if (P.shared > 0) {
+    float w = 1.f;
+    if (A.cols > A.experts) {
+      double s = l[A.experts];
+      // No part of a float sum leaves float's range where both squared norms are in it
+      // (it is at most their root); elsewhere the sum in double, as few rows have it.
+      if (P.norms && !(P.norms[A.cols + t] < INFINITY && P.norms[A.experts] < INFINITY)) {
+        const int e[EXACT] = {A.experts, A.experts};
+        s = exact_logits(A, t, e, lane);
+      }
+      w = sigmoid_f((float)s);
+    }
+    if (lane < P.shared) P.weights[(long)t * P.ld_w + P.top_k + lane] = w;
+  }
 }
 
 // One wave per token: a chain of a load, a search and a ranking (moe_topk.h) and, for
