@@ -6,6 +6,8 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import ffn_oracle as fo
 from margins import record
@@ -82,3 +84,43 @@ def test_shared_gate_beyond_floats_range(gpu, dtype, t, e):
     assert record("bound", fo.within(got[pick], want, bound, dtype), 1.0) <= 1.0
     for r in pick:
         assert record("alone", fo.within(gpu.moe(x[r:r + 1], w)[0], want[pick.index(r)], bound[pick.index(r)], dtype), 1.0) <= 1.0
+
+
+def calls(qm, seed=21):
+    """(name, call on x [rows, 96] bf16) of every operator that takes activations."""
+    router, mats, shared, row = layer_tensors(seed, 8, 96, 64, 1, BF16)
+    q = qm.mx4_quantize(mats[0][0])
+    w = qm.MoeWeights(router, *mats, top_k=2, shared=shared, shared_router=row)
+    return [("linear", lambda x: qm.mx4_linear(x, q)), ("sections", lambda x: qm.mx4_linear(x, q, sections=[60, 4])[1]),
+            ("route", lambda x: qm.moe_route(x, router, 2)[1]), ("moe", lambda x: qm.moe(x, w)),
+            ("quantize", lambda x: qm.mx4_quantize(x).dequantize())]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("t", [1, 20])
+def test_derivatives_and_traces_are_refused(gpu, t):
+    x = normal(t, t, 96, dtype=BF16)
+    for name, call in calls(gpu):
+        want = call(x)
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(fw.make_dual(x, torch.ones_like(x)))
+            assert torch.equal(call(x), want), name
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(call)(x)
+        for f in (lambda v: torch.func.jvp(call, (v,), (v,)), torch.func.grad(lambda v: call(v).float().sum()),
+                  lambda v: torch.vmap(call)(v[None])):
+            with pytest.raises(RuntimeError):
+                f(x)
+        assert torch.equal(call(x), want), name
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_calls_inside_a_compiled_function(gpu):
+    x = normal(3, 20, 96, dtype=BF16)
+    for name, call in calls(gpu):
+        compiled = torch.compile(lambda v: call(v * 2) + 1, backend="eager")
+        for _ in range(2):
+            assert torch.equal(compiled(x), call(x * 2) + 1), name

@@ -10,8 +10,11 @@ projections in it, ``MoeWeights`` a mixture-of-experts layer's.
 
 The weights live on the device in the matrix cores' operand order
 (include/qwen4mix.h); everything runs in the HIP kernels of libqwen4mix.so, on
-the current stream of the tensors' device. Nothing here is differentiable:
-inputs that require a gradient are refused while gradients are recorded.
+the current stream of the tensors' device. Nothing here is differentiable or
+traceable: inputs that require a gradient are refused while gradients are
+recorded, inputs with a tangent always, and so is any call while torch.jit.trace
+or make_fx records (torch.compile breaks its graph around the calls). Autocast
+casts nothing: outputs have their input's type.
 """
 
 from __future__ import annotations
@@ -19,6 +22,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -28,10 +32,20 @@ TILE_ROWS, TILE_K = 16, 128
 
 _ACT = {torch.float32: native.QM_ACT_F32, torch.bfloat16: native.QM_ACT_BF16}
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+
+
+def refuse_recording() -> None:
+    """Raise where torch records the operations of a call: it would see the output
+    made and not what the kernels write into it."""
+    if _tracing_state() is not None or _dispatch_modes() and \
+            torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("the 4-bit weights' and the experts' operators cannot be traced (torch.jit.trace, make_fx)")
 
 
 def launch(name: str, device, *args) -> None:
     """The entry point ``name`` on ``args`` and the current stream of ``device``."""
+    refuse_recording()
     fn, index = getattr(native.load(), name), device.index
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
@@ -44,7 +58,9 @@ def launch(name: str, device, *args) -> None:
 
 def check_input(t: torch.Tensor, what: str) -> int:
     """The type code of a float32 or bfloat16 tensor on the GPU that loses no
-    gradient here."""
+    gradient or tangent here."""
+    if forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{what} has a tangent, and this operator has no forward derivative")
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a tensor on the GPU")
     if t.requires_grad and torch.is_grad_enabled():
