@@ -477,7 +477,8 @@ int qm_hc_reinject(const qm_hc_geom* g, const void* hyper, const void* branch, c
  * of 16 rows x 128 k, [matrix][ceil(n/16)][ceil(k/128)]: codes of 1024 bytes a
  * tile, where 16-byte slot l holds block l / 16 of row l % 16 (element j in
  * nibble j, the low nibble of a byte first), and scales of 64 bytes a tile, byte
- * l for slot l. Slots past n or k are zero. codes are 16-byte aligned. */
+ * l for slot l. Slots past n or k are zero. codes are 16-byte aligned, scales that
+ * are multiplied 4-byte aligned. */
 
 /* Bytes of the codes of `mats` matrices (the scales take a 16th of it); 0 if the
  * sizes are unsupported. */
@@ -505,7 +506,8 @@ int qm_mx4_layout(int to_tiles, int mats, int n, int k, void* codes, void* scale
  * activation rows: y[m][j] = sum_k w[j][k] x[m][k], w the values the codes stand
  * for, float sums rounded once to act_dtype.
  *   x [m, k] act_dtype, rows ldx elements apart (ldx >= k, whole 16-byte units;
- *   x 16-byte aligned); segments as qm_gemv. Outputs may not overlap x. */
+ *   x 16-byte aligned); scales 4-byte aligned; segments as qm_gemv. Outputs may not
+ *   overlap x. */
 int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* codes, const void* scales, const void* x, long ldx,
                   int n_seg, const int* seg_rows, void* const* seg_out, hipStream_t stream);
 
@@ -575,8 +577,8 @@ size_t qm_moe_workspace(const qm_moe_geom* g);
  * with ids and w as qm_moe_route. Products accumulate in float; a pair's weighted
  * hidden row is rounded to act_dtype between them, the output once.
  *   x [rows, hidden] act, rows ldx elements apart; out [rows, hidden] act; every
- *   pointer 16-byte aligned. out may not overlap x. The workspace holds nothing
- *   between calls; calls that overlap need one each. */
+ *   pointer 16-byte aligned, scales 4-byte. out may not overlap x. The workspace holds
+ *   nothing between calls; calls that overlap need one each. */
 int qm_moe(const qm_moe_geom* g, const qm_moe_weights* w, const void* x, long ldx, void* out, void* workspace,
            size_t workspace_bytes, hipStream_t stream);
 

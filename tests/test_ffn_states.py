@@ -1,7 +1,9 @@
-"""Host-side checks of the experts' and the 4-bit weights' Python layer that need no
-GPU: what it refuses before any tensor is read."""
+"""Host-side checks of the experts' and the 4-bit weights' entry points that need no
+GPU: what they refuse before any tensor is read."""
 
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 import torch
@@ -42,3 +44,22 @@ def test_recording_is_refused(qm):
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda v: (mx4.launch("qm_mx4_quantize", None), v + 1)[1], x)
     f(x)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("m", [1, 200])
+def test_scales_that_are_not_whole_words_are_refused(qm, m, off):
+    """For the few-row kernels, which read bytes, as for the staged ones, which read
+    words."""
+    n = qm.native
+    lib = n.load()
+    p = ctypes.c_void_p(64)
+    seg, out = (ctypes.c_int * 1)(4096), (ctypes.c_void_p * 1)(64)
+    assert lib.qm_mx4_linear(1, m, 4096, 64, p, ctypes.c_void_p(64 + off), p, 64, 1, seg, out, None) == -1
+    assert b"scales" in lib.qm_last_error()
+    g = n.MoeGeom(m, 64, 32, 8, 1, 2, 1, 1, n.QM_W_MX4)
+    for name in ("gate", "up", "down", "shared_gate", "shared_up", "shared_down"):
+        w = n.MoeWeightPtrs(*([64] * 14))
+        setattr(w, name + "_scales", 64 + off)
+        assert lib.qm_moe(ctypes.byref(g), ctypes.byref(w), p, 64, p, p, 1 << 30, None) == -1, name
+        assert b"scales" in lib.qm_last_error()

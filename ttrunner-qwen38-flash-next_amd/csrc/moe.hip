@@ -705,7 +705,8 @@ extern "C" int qm_moe(const qm_moe_geom* g, const qm_moe_weights* w, const void*
     if (!need[i] || !aligned16(need[i])) return qm_fail(QM_ERR_ARG, "qm_moe: a weight is null or not 16-byte aligned");
   if (g->weight_format == QM_W_MX4)
     for (int i = 0; i < (g->shared ? 6 : 3); ++i)
-      if (!scales[i]) return qm_fail(QM_ERR_ARG, "qm_moe: null scales");
+      if (!scales[i] || reinterpret_cast<uintptr_t>(scales[i]) & 3)
+        return qm_fail(QM_ERR_ARG, "qm_moe: scales are null or not 4-byte aligned");
   if (!aligned16(x) || !aligned16(out) || !aligned16(workspace) || (w->shared_router && !aligned16(w->shared_router)))
     return qm_fail(QM_ERR_ARG, "qm_moe: x, out, workspace and shared_router must be 16-byte aligned");
   const MoeLayout l = moe_layout(*g);

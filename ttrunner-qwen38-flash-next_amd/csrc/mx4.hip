@@ -440,6 +440,8 @@ extern "C" int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* cod
   const int unit = act_dtype == QM_ACT_BF16 ? 8 : 4;
   if (ldx < k || ldx % unit) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: ldx must be at least k and whole 16-byte units");
   if (!aligned16(codes) || !aligned16(x)) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: codes and x must be 16-byte aligned");
+  // (the staged kernels load them four at a time)
+  if (reinterpret_cast<uintptr_t>(scales) & 3) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: scales must be 4-byte aligned");
   if (n_seg <= 0 || n_seg > QM_GEMV_MAX_SEG) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: 1..8 output segments");
   for (int s = 0; s < n_seg; ++s)
     if (seg_rows[s] <= 0 || !seg_out[s]) return qm_fail(QM_ERR_ARG, "qm_mx4_linear: empty segment or null output");
