@@ -3,7 +3,9 @@ GPU: what they refuse before any tensor is read."""
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -63,3 +65,19 @@ def test_scales_that_are_not_whole_words_are_refused(qm, m, off):
         setattr(w, name + "_scales", 64 + off)
         assert lib.qm_moe(ctypes.byref(g), ctypes.byref(w), p, 64, p, p, 1 << 30, None) == -1, name
         assert b"scales" in lib.qm_last_error()
+
+
+def test_weights_do_not_change_once_made(qm):
+    """Calls keep their addresses and sizes."""
+    q = qm.Mx4Weight(torch.zeros(4 * 1088, dtype=torch.uint8), (17, 160))
+    w = qm.MoeWeights.__new__(qm.MoeWeights)
+    w.top_k = 2
+    for obj, name, value in ((q, "data", torch.zeros(1088, dtype=torch.uint8)), (q, "shape", (16, 32)), (q, "code_bytes", 1),
+                             (w, "top_k", 3)):
+        with pytest.raises(AttributeError, match="does not change"):
+            setattr(obj, name, value)
+        with pytest.raises(AttributeError, match="does not change"):
+            delattr(obj, name)
+    assert q.data.numel() == 4 * 1088 and w.top_k == 2
+    for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert other.shape == q.shape and torch.equal(other.data, q.data)

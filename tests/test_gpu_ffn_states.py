@@ -4,6 +4,8 @@ beyond float's range, very wide weights, skewed routers."""
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -124,3 +126,24 @@ def test_calls_inside_a_compiled_function(gpu):
         compiled = torch.compile(lambda v: call(v * 2) + 1, backend="eager")
         for _ in range(2):
             assert torch.equal(compiled(x), call(x * 2) + 1), name
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+def test_a_layer_does_not_change_once_made(gpu, fmt):
+    """What a call of some row count keeps holds for every other: nothing of it can be
+    replaced."""
+    router, mats, shared, row = layer_tensors(31, 8, 96, 64, 1, BF16)
+    lay = gpu.mx4_quantize if fmt == "mx4" else (lambda m: m)
+    w = gpu.MoeWeights(router, *(lay(m) for m in mats), top_k=2, shared=[lay(m) for m in shared], shared_router=row)
+    x = normal(32, 40, 96, dtype=BF16)
+    want = gpu.moe(x, w)
+    for name, value in (("top_k", 3), ("normalize", False), ("router", router), ("down", w.up), ("shared", 0),
+                        ("shared_router", None), ("s_down", None), ("hidden", 64), ("ptrs", None)):
+        with pytest.raises(AttributeError, match="does not change"):
+            setattr(w, name, value)
+    for part in (w.gate, w.down, w.s_up):
+        with pytest.raises(AttributeError, match="does not change"):
+            part.data = part.data.clone()
+    assert torch.equal(gpu.moe(x, w), want)
+    other = copy.copy(w)                                            # a shallow copy shares the memory
+    assert torch.equal(gpu.moe(x, other), want) and other.down.data.data_ptr() == w.down.data.data_ptr()

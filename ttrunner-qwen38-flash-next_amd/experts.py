@@ -18,7 +18,7 @@ import functools
 import torch
 
 from . import native
-from .mx4 import BLOCK, Mx4Weight, activation_rows, check_input, dense, launch
+from .mx4 import BLOCK, Mx4Weight, SetOnce, activation_rows, check_input, dense, launch
 
 MAX_EXPERTS, MAX_TOP_K, MAX_SHARED = 1024, 32, 32
 
@@ -81,7 +81,7 @@ def _copy(t: torch.Tensor) -> torch.Tensor:
     return t.detach().clone(memory_format=torch.contiguous_format)
 
 
-class _Tiles:
+class _Tiles(SetOnce):
     """A weight [mats, n, k] of the activations' type in the kernels' tile order."""
 
     def __init__(self, w: torch.Tensor):
@@ -99,7 +99,7 @@ class _Tiles:
         return self.data.data_ptr()
 
 
-class MoeWeights:
+class MoeWeights(SetOnce):
     """The weights of a mixture-of-experts layer, copied and laid out once for the
     kernels (an ``Mx4Weight`` is such a copy already and is kept as it is).
 
@@ -108,7 +108,8 @@ class MoeWeights:
     that type or ``Mx4Weight``s, and so is ``shared``, the (gate, up, down) of the
     experts that every token takes (leading dimension: how many, each as wide as
     a routed one), behind the sigmoid of ``shared_router`` [hidden] when that is
-    given. ``normalize``: a token's routed weights add up to 1."""
+    given. ``normalize``: a token's routed weights add up to 1. Its attributes do not
+    change: another ``top_k`` is another ``MoeWeights``."""
 
     def __init__(self, router, gate, up, down, top_k: int, shared=None, shared_router=None, normalize: bool = True):
         _check_router_shape(router)
@@ -124,21 +125,22 @@ class MoeWeights:
         if self.inter == 0 or self.inter % BLOCK:
             raise ValueError(f"the experts' width must be a multiple of {BLOCK}, got {self.inter}")
         self.gate, self.up, self.down = self._take(self.experts, (gate, up, down), "")
-        self.shared = 0
-        self.s_gate = self.s_up = self.s_down = self.shared_router = None
+        count, parts, row = 0, (None, None, None), None
         if shared is not None:
-            self.shared = int(shared[0].shape[0])
-            if not 1 <= self.shared <= MAX_SHARED:
-                raise ValueError(f"1 to {MAX_SHARED} shared experts, got {self.shared}")
-            self.s_gate, self.s_up, self.s_down = self._take(self.shared, shared, "shared ")
+            count = int(shared[0].shape[0])
+            if not 1 <= count <= MAX_SHARED:
+                raise ValueError(f"1 to {MAX_SHARED} shared experts, got {count}")
+            parts = self._take(count, shared, "shared ")
             if shared_router is not None:
                 check_input(shared_router, "shared_router")
                 if shared_router.numel() != self.hidden or shared_router.dtype != router.dtype \
                         or shared_router.device != router.device:
                     raise ValueError(f"shared_router must be [{self.hidden}] in {router.dtype} on {router.device}")
-                self.shared_router = _copy(shared_router.reshape(-1))
+                row = _copy(shared_router.reshape(-1))
         elif shared_router is not None:
             raise ValueError("shared_router without shared experts")
+        self.shared, self.shared_router = count, row
+        self.s_gate, self.s_up, self.s_down = parts
         self._bind()
 
     def _bind(self) -> None:

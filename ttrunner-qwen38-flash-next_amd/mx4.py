@@ -90,16 +90,33 @@ def activation_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return dense(rows), k
 
 
-class Mx4Weight:
+class SetOnce:
+    """Attributes that are set once: calls, decoders and captured graphs keep the
+    addresses and sizes that they stand for."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} does not change: make a new one")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} does not change: make a new one")
+
+
+class Mx4Weight(SetOnce):
     """A weight [..., n, k] in 4-bit blocks along k, laid out for the kernels.
 
-    ``data`` holds the device tiles, ``codes`` and ``scales`` are views of it;
-    ``plain()`` gives them in a checkpoint's order, ``dequantize()`` the values they
-    stand for."""
+    ``data`` holds the device tiles (uint8, 17 bytes for 32 weights of tiles of 16
+    rows x 128 k), ``codes`` and ``scales`` are views of it; ``plain()`` gives them in
+    a checkpoint's order, ``dequantize()`` the values they stand for. Made by
+    ``mx4_quantize`` or ``from_codes``; its attributes do not change."""
 
     def __init__(self, data: torch.Tensor, shape):
-        self.data, self.shape = data, shape if type(shape) is torch.Size else torch.Size(shape)
-        self.mats = 1 if len(shape) == 2 else self.shape[:-2].numel()
+        self._set(data, torch.Size(shape))
+
+    def _set(self, data: torch.Tensor, shape: torch.Size) -> None:
+        self.data, self.shape = data, shape
+        self.mats = 1 if len(shape) == 2 else shape[:-2].numel()
         # the codes are 16 of 17 bytes, the scales behind them
         self.code_bytes = data.numel() // 17 * 16
 
@@ -132,13 +149,19 @@ class Mx4Weight:
             raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {shape[-1]}")
 
     @classmethod
-    def _empty(cls, shape, device) -> "Mx4Weight":
+    def _bytes(cls, shape: torch.Size) -> int:
         cls._check_shape(shape)
         n, k = shape[-2:]
         tiles = -(-n // TILE_ROWS) * -(-k // TILE_K)
         if len(shape) > 2:
             tiles *= shape[:-2].numel()
-        return cls(torch.empty(tiles * (TILE_ROWS * TILE_K // 32 * 17), dtype=torch.uint8, device=device), shape)
+        return tiles * (TILE_ROWS * TILE_K // 32 * 17)
+
+    @classmethod
+    def _empty(cls, shape: torch.Size, device) -> "Mx4Weight":
+        w = cls.__new__(cls)
+        w._set(torch.empty(cls._bytes(shape), dtype=torch.uint8, device=device), shape)
+        return w
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mx4Weight":
