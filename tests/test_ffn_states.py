@@ -67,6 +67,19 @@ def test_scales_that_are_not_whole_words_are_refused(qm, m, off):
         assert b"scales" in lib.qm_last_error()
 
 
+def test_a_4_bit_weight_is_as_large_as_its_shape(qm):
+    """Tiles that a kernel would read past are refused where the weight is made."""
+    tiles = lambda n: torch.zeros(n * 1088, dtype=torch.uint8)  # noqa: E731
+    assert qm.Mx4Weight(tiles(4), (17, 160)).code_bytes == 4 * 1024
+    assert qm.Mx4Weight(tiles(12), (3, 17, 160)).mats == 3
+    for data, shape in ((tiles(3), (17, 160)), (tiles(5), (17, 160)), (tiles(4), (3, 17, 160)), (tiles(4).int(), (17, 160)),
+                        (tiles(8)[::2], (17, 160)), (torch.zeros(4 * 1088 + 1, dtype=torch.uint8)[1:], (17, 160))):
+        with pytest.raises(ValueError, match="tiles of"):
+            qm.Mx4Weight(data, shape)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        qm.Mx4Weight(tiles(4), (17, 150))
+
+
 def test_weights_do_not_change_once_made(qm):
     """Calls keep their addresses and sizes."""
     q = qm.Mx4Weight(torch.zeros(4 * 1088, dtype=torch.uint8), (17, 160))

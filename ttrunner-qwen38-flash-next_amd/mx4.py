@@ -112,7 +112,12 @@ class Mx4Weight(SetOnce):
     ``mx4_quantize`` or ``from_codes``; its attributes do not change."""
 
     def __init__(self, data: torch.Tensor, shape):
-        self._set(data, torch.Size(shape))
+        shape = torch.Size(shape)
+        need = self._bytes(shape)
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != need or data.data_ptr() % 16:
+            raise ValueError(f"the tiles of {tuple(shape)} are {need} bytes (uint8, contiguous, 16-byte aligned), got "
+                             f"{data.dtype} {tuple(data.shape)}")
+        self._set(data, shape)
 
     def _set(self, data: torch.Tensor, shape: torch.Size) -> None:
         self.data, self.shape = data, shape
