@@ -94,3 +94,10 @@ def test_weights_do_not_change_once_made(qm):
     assert q.data.numel() == 4 * 1088 and w.top_k == 2
     for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
         assert other.shape == q.shape and torch.equal(other.data, q.data)
+
+
+def test_the_experts_fields_stand_behind_the_configurations_others(qm):
+    """Configurations made by position keep their meaning."""
+    c = qm.MixConfig(1024, 1e-5, 8, 1, 128, 1e6, 32, [6, 5, 5], 2, 2, 64, 512, 32, 16, 8, 64, 3, "sigmoid", 2, 160, 128)
+    assert (c.hc_count, c.hc_lowrank, c.page_size) == (2, 160, 128)
+    assert (c.num_experts_per_tok, c.norm_topk_prob, c.shared_expert) == (8, True, True)

@@ -37,10 +37,10 @@ class MixConfig:
     output_gate_type: str = "sigmoid"
     hc_count: int = 4
     hc_lowrank: int = 320
+    page_size: int = 64
     num_experts_per_tok: int = 8
     norm_topk_prob: bool = True
     shared_expert: bool = True
-    page_size: int = 64
 
     @property
     def hc_hidden_size(self) -> int:
