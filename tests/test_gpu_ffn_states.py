@@ -147,3 +147,19 @@ def test_a_layer_does_not_change_once_made(gpu, fmt):
     assert torch.equal(gpu.moe(x, w), want)
     other = copy.copy(w)                                            # a shallow copy shares the memory
     assert torch.equal(gpu.moe(x, other), want) and other.down.data.data_ptr() == w.down.data.data_ptr()
+
+
+# Few rows of weights so wide that they alone make more workgroups than the chip holds:
+# both sides of each border of the choice of kernel (8 | 9, 16 | 17 and 32 | 33 rows), and
+# of the widths where it begins (bf16 32768 and 196608 rows of weights, float 131072).
+@pytest.mark.parametrize("dtype,n", [(BF16, 32700), (BF16, 33001), (BF16, 196700), (F32, 130900), (F32, 131100)])
+@pytest.mark.parametrize("m", [1, 8, 9, 16, 17, 32, 33])
+def test_few_rows_of_a_wide_weight(gpu, dtype, n, m):
+    k = 160
+    q = gpu.mx4_quantize(normal(n, n, k, dtype=dtype, scale=k ** -0.5))
+    x = normal(m, m, k, dtype=dtype)
+    want, bound = fo.linear(x, q.dequantize(F32))
+    got = gpu.mx4_linear(x, q)
+    assert record("bound", fo.within(got, want, bound, dtype), 1.0) <= 1.0
+    parts = gpu.mx4_linear(x, q, sections=[n - 1000, 999, 1])
+    assert torch.equal(torch.cat(parts, -1), got)

@@ -306,16 +306,25 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
 //     (776) - / 30.5 / 22.9 / 20.0 / 21.2, 512 rows (1552) - / 52 / 40 / 37 / 33.5; 9856
 //     x 2048: 400 rows (1001) 39 / 31 / 23.7 / 21.1 / 29.7; 2048 x 4096: 256 rows (128)
 //     10.4 / 13.4 / 15.4 / 23.0 / 35, 400 rows (208) 16.6 / 13.6 / 15.3 / 19.7 / 35
+//     Wide weights, whose few rows make as many workgroups: up to 8 rows stay with the
+//     few-row kernel, up to 32 with tiles of 32 (few-row / 256 x 32 / 256 x 64, x 2048:
+//     65536, 1 row 16.8 / 19.3 / 20.7; 151936: 1 row 33.1 / 35.6 / 47.4, 8 rows 34.9 /
+//     35.9 / 49.7, 16 rows 38.6 / 36.6 / 52.1, 32 rows 60 / 40.8 / 56.8; 262144: 1 row
+//     51.7 / 61.8 / 63.3, 8 rows 54.0 / 63.1 / 66.0, 32 rows 120 / 66.2 / 73.0)
 //   float   256 x 32 tiles from 512 workgroups on (2000 rows of 9856 x 2048: 283
-//     against 328; 256 of 12352 x 2048, 392 of them: 60 against 63)
+//     against 328; 256 of 12352 x 2048, 392 of them: 60 against 63), but for up to 16
+//     rows of a wide weight, which keep four row tiles a workgroup (four / eight / 256 x
+//     32, x 2048: 65536, 1 row 22.1 / 23.9 / 41; 151936: 1 row 49 / 53 / 91, 16 rows 53 /
+//     56 / 96, 17 rows 89 / 100 / 97; 262144: 1 row 76 / 83 / 119, 17 rows 148 / 162 / 130)
 template <typename T>
 int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   auto groups = [&A](int bn, int bm) { return (long)((A.rt * 16 + bn - 1) / bn) * ((A.m + bm - 1) / bm); };
   if constexpr (sizeof(T) == 2) {
     if (groups(64, 16) > 512) {
+      if (A.m <= 8) return launch_rows<T, 4, 8>(A, stream);
       if (groups(128, 32) <= 256) return launch_gemm<T, 2, 2, 4, 1, 2, 4>(A, stream);
       if (groups(128, 32) <= 640) return launch_gemm<T, 2, 2, 4, 1, 2, 2>(A, stream);
-      if (groups(256, 32) <= 768) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
+      if (groups(256, 32) <= 768 || A.m <= 32) return launch_gemm<T, 2, 2, 8, 1, 2>(A, stream);
       return launch_gemm<T, 2, 4, 8, 1, 2>(A, stream);
     }
     if (groups(16, 16) <= 256) return launch_rows<T, 1, 16>(A, stream);
@@ -323,10 +332,10 @@ int run_linear(const Mx4LinearArgs<T>& A, hipStream_t stream) {
     if (groups(32, 16) <= 512) return launch_rows<T, 2, 8>(A, stream);
     return launch_rows<T, 4, 8>(A, stream);
   } else {
-    if (groups(256, 32) >= 512) return launch_gemm<T, 4, 2, 4, 1, 2>(A, stream);
+    if (groups(256, 32) >= 512 && A.m > 16) return launch_gemm<T, 4, 2, 4, 1, 2>(A, stream);
     if (groups(16, 16) <= 256) return launch_rows<T, 1, 16>(A, stream);
     if (groups(32, 16) <= 256) return launch_rows<T, 2, 16>(A, stream);
-    if (groups(64, 16) <= 256) return launch_rows<T, 4, 8>(A, stream);
+    if (groups(64, 16) <= 256 || A.m <= 16) return launch_rows<T, 4, 8>(A, stream);
     return launch_rows<T, 8, 8>(A, stream);
   }
 }
