@@ -163,3 +163,18 @@ def test_few_rows_of_a_wide_weight(gpu, dtype, n, m):
     assert record("bound", fo.within(got, want, bound, dtype), 1.0) <= 1.0
     parts = gpu.mx4_linear(x, q, sections=[n - 1000, 999, 1])
     assert torch.equal(torch.cat(parts, -1), got)
+
+
+# Both sides of the products up to which every logit is summed in double. A weight is
+# within 2^-18 of the softmax of those sums (an exponential of a difference below 16
+# rounded to float, a float sum, a division), and by 4 B more where the matrix cores
+# sum 128 products at a time: B = (129 2^-23) |x| |R[e]| bounds their error.
+@pytest.mark.parametrize("dtype,t,e,h", [(BF16, 755, 64, 2048), (BF16, 770, 64, 2048), (F32, 2800, 64, 2048),
+                                         (F32, 2850, 64, 2048)])
+def test_route_at_the_border_of_its_sums(gpu, dtype, t, e, h):
+    x, r = normal(t, t, h, dtype=dtype), normal(h, e, h, dtype=dtype, scale=h ** -0.5)
+    ids, w = gpu.moe_route(x, r, 6)
+    want_ids, want_w = fo.route(x, r, 6)
+    assert torch.equal(ids, want_ids)
+    lim = 2.0 ** -18 + 4 * 129 * 2.0 ** -23 * x.double().norm(dim=-1) * r.double().norm(dim=-1).max()
+    assert record("bound", ((w.double() - want_w).abs() / want_w / lim[:, None]).max().item(), 1.0) <= 1.0

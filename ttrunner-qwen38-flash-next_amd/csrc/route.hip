@@ -21,10 +21,12 @@
 namespace {
 
 // Products of a call (rows x columns x hidden) up to which every logit is summed in
-// double. Logits and choice of 128 experts over 2048, us, so / by matrix cores: bf16
-// 256 rows (7e7) 17 / 22, 360 rows 21 / 23, 460 rows (1.2e8) 25 / 22, 1000 rows 44 /
-// 23; float 1024 rows (2.7e8) 53 / 70, 1500 rows (3.9e8) 73 / 70, 2048 rows 98 / 70.
-template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 4e8;
+// double. Logits and choice over 2048, us, so / by matrix cores: bf16 128 experts 256
+// rows (7e7) 16 / 20, 330 rows (9e7) 20 / 20, 400 rows (1.05e8) 22 / 21; float 128
+// experts 1250 rows (3.3e8) 62 / 70, 1400 rows (3.7e8) 69 / 70, 1500 rows (3.9e8) 74 /
+// 70; 256 experts 700 rows (3.7e8) 69 / 71, 800 rows 78 / 69; 64 experts 2800 rows
+// (3.7e8) 70 / 70, 3000 rows 76 / 70.
+template <typename T> constexpr double ROUTE_FEW = sizeof(T) == 2 ? 1e8 : 3.7e8;
 // Choices of an expert, on average, up to which the choosing waves file them by
 // atomics (they serialise: 8 each +2.4 us, 16 +4.2, 32 +7.2, 250 +31); beyond, a
 // launch of its own does (6.0 us and its start, 7.7 at 16000 choices)
