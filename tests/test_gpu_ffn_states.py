@@ -178,3 +178,123 @@ def test_route_at_the_border_of_its_sums(gpu, dtype, t, e, h):
     assert torch.equal(ids, want_ids)
     lim = 2.0 ** -18 + 4 * 129 * 2.0 ** -23 * x.double().norm(dim=-1) * r.double().norm(dim=-1).max()
     assert record("bound", ((w.double() - want_w).abs() / want_w / lim[:, None]).max().item(), 1.0) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_read_back_of_every_code_and_scale(gpu, dtype):
+    """All 16 codes under all 256 scales: subnormal values are exact, those past the
+    type's range infinite, scale 255 NaN."""
+    codes = torch.arange(16, dtype=torch.uint8, device=DEV)
+    codes = (codes | codes.flip(0) << 4).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.uint8, device=DEV)[:, None]
+    q = gpu.Mx4Weight.from_codes(codes, scales)
+    got, want = q.dequantize(dtype), fo.mx4_decode(codes, scales)
+    assert torch.equal(got[:255].double(), want[:255].to(dtype).double())
+    assert torch.equal(torch.signbit(got[:255]), torch.signbit(want[:255])) and bool(got[255].isnan().all())
+    tiny = want[0].abs()[want[0] != 0].min().item()
+    assert tiny == 2.0 ** -128 and got[0].double().abs()[got[0] != 0].min().item() == tiny
+    back = q.plain()
+    assert torch.equal(back[0], codes) and torch.equal(back[1], scales)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n", [(2, 70), (9, 70), (40, 300), (60, 4090), (170, 4090), (300, 4090), (700, 4090),
+                                 (2000, 1000), (5, 33000), (20, 33000)])
+def test_an_infinite_activation_reaches_every_output(gpu, dtype, m, n):
+    """inf times a weight is that infinity, inf times zero is NaN: no output of the row
+    stays finite, whichever kernel has it."""
+    k = 224
+    w = normal(n, n, k, dtype=dtype)
+    w[::7, k - 1] = 0
+    q = gpu.mx4_quantize(w)
+    column = q.dequantize(F32)[:, k - 1]
+    assert bool((column == 0).any()) and bool((column > 0).any()) and bool((column < 0).any())
+    x = normal(m, m, k, dtype=dtype)
+    clean = gpu.mx4_linear(x, q)
+    x[0, k - 1], x[m - 1, k - 1] = float("inf"), float("-inf")
+    got = gpu.mx4_linear(x, q)
+    for row, sign in ((0, 1.0), (m - 1, -1.0)):
+        assert not bool(got[row].isfinite().any())
+        assert torch.equal(got[row].isnan(), column == 0)
+        hit = column != 0
+        assert torch.equal(torch.sign(got[row].float())[hit], sign * torch.sign(column)[hit])
+    assert torch.equal(got[1:m - 1], clean[1:m - 1])
+
+
+def make(qm, tensors, fmt, top_k, normalize=True):
+    """(MoeWeights, the oracle's arguments) of layer_tensors."""
+    router, mats, shared, row = tensors
+    shared = shared if shared[0].shape[0] else None
+    if fmt == "mx4":
+        mats, shared = [qm.mx4_quantize(m) for m in mats], None if shared is None else [qm.mx4_quantize(m) for m in shared]
+        value = lambda m: m.dequantize().double()  # noqa: E731
+    else:
+        value = lambda m: m.double()  # noqa: E731
+    row = None if shared is None else row
+    w = qm.MoeWeights(router, *mats, top_k=top_k, shared=shared, shared_router=row, normalize=normalize)
+    return w, dict(zip(("gate", "up", "down"), map(value, mats)), router=router, top_k=top_k, normalize=normalize,
+                   shared=None if shared is None else [value(m) for m in shared], shared_router=row)
+
+
+def check(got, x, args):
+    want, bound = fo.moe(x, **args)
+    assert got.shape == x.shape and got.dtype == x.dtype
+    assert record("bound", fo.within(got, want, bound, x.dtype), 1.0) <= 1.0
+
+
+# float layers at the borders between the kernels: 16 and 17 tokens; lists by the choosing
+# waves and apart, over several rounds of choices; weights read once and more often; logits
+# by matrix cores; then layers of many experts, of either type
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("dtype,t,e,k,h,i,shared", [
+    (F32, 16, 24, 4, 288, 160, 1), (F32, 17, 24, 4, 288, 160, 1), (F32, 300, 8, 2, 160, 96, 1), (F32, 90, 16, 2, 160, 96, 0),
+    (F32, 3000, 32, 6, 64, 32, 0), (F32, 6000, 60, 4, 1056, 32, 1), (F32, 40, 1024, 32, 32, 32, 0), (F32, 3, 32, 32, 64, 32, 32),
+    (BF16, 1, 256, 8, 512, 128, 1), (BF16, 50, 512, 10, 256, 64, 1), (BF16, 400, 256, 8, 256, 64, 0),
+    (F32, 12, 300, 6, 128, 64, 1), (BF16, 2000, 640, 4, 128, 32, 0)])
+def test_float_layers_and_many_experts(gpu, fmt, dtype, t, e, k, h, i, shared):
+    print(f"moe {dtype} {fmt} t={t} e={e} k={k} h={h} i={i} shared={shared}", flush=True)
+    w, args = make(gpu, layer_tensors(t + e, e, h, i, shared, dtype), fmt, k, normalize=t % 2 == 0)
+    x = normal(t, t, h, dtype=dtype)
+    check(gpu.moe(x, w), x, args)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,e,k", [(6, 64, 6), (16, 256, 8), (150, 64, 6), (900, 160, 4)])
+def test_skewed_routers(gpu, fmt, dtype, t, e, k):
+    """Load as trained routers have it: the tokens share a direction, and the experts'
+    rows follow it by falling amounts, so a few experts take most rows, most none."""
+    h, i = 160, 64
+    tensors = layer_tensors(41, e, h, i, 1, dtype)
+    shared_direction = normal(42, h)
+    order = torch.randperm(e, generator=torch.Generator().manual_seed(43)).to(DEV)
+    lean = 4.0 / (1.0 + order.float())
+    tensors[0].copy_(tensors[0] + (lean[:, None] * shared_direction * h ** -0.5).to(dtype))
+    x = normal(t, t, h, dtype=dtype) + shared_direction.to(dtype)
+    w, args = make(gpu, tensors, fmt, k)
+    ids = gpu.moe_route(x, tensors[0], k)[0]
+    counts = torch.bincount(ids.flatten().long(), minlength=e)
+    assert counts.max().item() > 0.8 * t
+    check(gpu.moe(x, w), x, args)
+
+
+def test_the_largest_calls(gpu):
+    """As many rows as one call takes, and one more."""
+    h, t = 32, 262140
+    w, args = make(gpu, layer_tensors(51, 4, h, 32, 0, BF16), "plain", 1)
+    x = normal(52, t + 1, h, dtype=BF16)
+    got = gpu.moe(x[:t], w)
+    want, bound = fo.moe(x[:t], **args)
+    assert record("bound", fo.within(got, want, bound, BF16), 1.0) <= 1.0
+    for call in (lambda: gpu.moe(x, w), lambda: gpu.moe_route(x, args["router"], 1)):
+        with pytest.raises(gpu.native.QmError, match="262140"):
+            call()
+    del got, want, bound
+    m = 16 * 65535
+    for dtype in (BF16, F32):
+        q = gpu.mx4_quantize(normal(53, 20, h, dtype=dtype))
+        x = normal(54, m + 1, h, dtype=dtype)
+        want, bound = fo.linear(x[:m], q.dequantize(F32))
+        assert record("bound", fo.within(gpu.mx4_linear(x[:m], q), want, bound, dtype), 1.0) <= 1.0
+        with pytest.raises(gpu.native.QmError, match="1048560"):
+            gpu.mx4_linear(x, q)
