@@ -5,6 +5,7 @@ beyond float's range, very wide weights, skewed routers."""
 from __future__ import annotations
 
 import copy
+import threading
 
 import pytest
 import torch
@@ -298,3 +299,31 @@ def test_the_largest_calls(gpu):
         assert record("bound", fo.within(gpu.mx4_linear(x[:m], q), want, bound, dtype), 1.0) <= 1.0
         with pytest.raises(gpu.native.QmError, match="1048560"):
             gpu.mx4_linear(x, q)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "mx4"])
+def test_calls_from_threads(gpu, fmt):
+    """Host threads with a stream each, every thread's first calls among them."""
+    e, h, i = 16, 256, 64
+    w, args = make(gpu, layer_tensors(61, e, h, i, 1, BF16), fmt, 4)
+    q = gpu.mx4_quantize(normal(62, 4000, h, dtype=BF16))
+    sizes = (1, 12, 90, 700)
+    xs = [[normal(70 + n, t, h, dtype=BF16) for t in sizes] for n in range(4)]
+    got = [None] * len(xs)
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[n] = [(gpu.moe(x, w), gpu.mx4_linear(x, q), *gpu.moe_route(x, args["router"], 4)) for _ in range(5) for x in xs[n]]
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for n, seq in enumerate(xs):
+        want = [(gpu.moe(x, w), gpu.mx4_linear(x, q), *gpu.moe_route(x, args["router"], 4)) for x in seq]
+        assert all(torch.equal(a, b) for rep in range(5) for one, ref in zip(got[n][rep * len(seq):], want)
+                   for a, b in zip(one, ref))

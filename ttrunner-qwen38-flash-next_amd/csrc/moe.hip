@@ -566,8 +566,10 @@ int launch_gemms(const MoeArgs<T>& A, long max_tiles, hipStream_t stream) {
   const int hn = TN / 2 * WN, dn = TN * WN;
   const long up = max_tiles * ((wt_row_tiles(A.inter) + hn - 1) / hn), down = max_tiles * ((wt_row_tiles(A.hidden) + dn - 1) / dn);
   if (up > 0x7fffffffL / NT || down > 0x7fffffffL / NT) return qm_fail(QM_ERR_UNSUPPORTED, "qm_moe: too many tiles for one launch");
-  int rc = qm_allow_lds(reinterpret_cast<const void*>(moe_up_gemm_kernel<WF, T, TN, TM, WN, WM, S, STREAM>), G::LDS_BYTES);
-  if (!rc) rc = qm_allow_lds(reinterpret_cast<const void*>(moe_down_gemm_kernel<WF, T, TN, TM, WN, WM, S, STREAM>), G::LDS_BYTES);
+  static std::atomic<uint64_t> up_ok{0}, down_ok{0};
+  int rc = qm_allow_lds(reinterpret_cast<const void*>(moe_up_gemm_kernel<WF, T, TN, TM, WN, WM, S, STREAM>), G::LDS_BYTES, up_ok);
+  if (!rc)
+    rc = qm_allow_lds(reinterpret_cast<const void*>(moe_down_gemm_kernel<WF, T, TN, TM, WN, WM, S, STREAM>), G::LDS_BYTES, down_ok);
   if (rc) return rc;
   hipLaunchKernelGGL((moe_up_gemm_kernel<WF, T, TN, TM, WN, WM, S, STREAM>), dim3((unsigned)up), dim3(NT), G::LDS_BYTES, stream, A);
   QM_CHECK_LAUNCH();

@@ -279,7 +279,8 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
   constexpr int NT = 64 * WN * WM * KS;
   const long nb = (long)((A.rt + TN * WN - 1) / (TN * WN)) * ((A.m + G::BM - 1) / G::BM);
   if (nb > 0x7fffffffL / NT) return qm_fail(QM_ERR_UNSUPPORTED, "qm_mx4_linear: too many tiles for one launch");
-  const int rc = qm_allow_lds(reinterpret_cast<const void*>(mx4_gemm_kernel<T, TN, TM, WN, WM, S, KS>), G::LDS_BYTES);
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = qm_allow_lds(reinterpret_cast<const void*>(mx4_gemm_kernel<T, TN, TM, WN, WM, S, KS>), G::LDS_BYTES, allowed);
   if (rc) return rc;
   hipLaunchKernelGGL((mx4_gemm_kernel<T, TN, TM, WN, WM, S, KS>), dim3((unsigned)nb), dim3(NT), G::LDS_BYTES, stream, A);
   QM_CHECK_LAUNCH();

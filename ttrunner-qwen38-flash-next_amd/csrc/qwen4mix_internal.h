@@ -2,6 +2,9 @@
 #pragma once
 
 #include <stddef.h>
+#include <stdint.h>
+
+#include <atomic>
 
 #include "qwen4mix.h"
 
@@ -46,9 +49,10 @@ int qm_dn_rule_chunk(int act_dtype, int batch, int seq, int heads, int hk, long 
 // occupancy per compute unit times the compute units. Cached per device.
 int qm_resident_workgroups(const void* kernel, int block_threads, size_t dyn_lds, int* out);
 
-// Let `kernel` use dyn_lds bytes of dynamic LDS on the current device (needed
-// once per kernel and device above 64 KB; remembered).
-int qm_allow_lds(const void* kernel, size_t dyn_lds);
+// Let `kernel` use dyn_lds bytes of dynamic LDS on the current device: needed once
+// per kernel and device above 64 KB, and remembered in `devices`, the kernel's own
+// (a bit per device, none at first; it always asks for the same bytes).
+int qm_allow_lds(const void* kernel, size_t dyn_lds, std::atomic<uint64_t>& devices);
 
 // Zero n_words 32-bit words at p with a fill kernel on `stream`.
 int qm_zero_words(void* p, long n_words, hipStream_t stream);

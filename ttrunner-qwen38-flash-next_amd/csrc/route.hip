@@ -510,7 +510,8 @@ int qm_route(const QmLogits<T>& A, int top_k, int normalize, int* ids, float* we
   } else {
     P.norms = norms;
     const size_t lds = (size_t)2 * LG_SPANS<T> * LG_ROWS * WT_K * sizeof(T);
-    rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds);
+    static std::atomic<uint64_t> allowed{0};
+    rc = qm_allow_lds(reinterpret_cast<const void*>(moe_logits_mma_kernel<T>), lds, allowed);
     if (rc) return rc;
     hipLaunchKernelGGL(moe_logits_mma_kernel<T>, dim3((A.cols + 63) / 64 * ((A.rows + 63) / 64)), dim3(512), lds, stream, A, norms);
     QM_CHECK_LAUNCH();

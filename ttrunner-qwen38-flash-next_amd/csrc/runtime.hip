@@ -66,10 +66,15 @@ int qm_resident_workgroups(const void* kernel, int block_threads, size_t dyn_lds
   return QM_OK;
 }
 
-int qm_allow_lds(const void* kernel, size_t dyn_lds) {
+int qm_allow_lds(const void* kernel, size_t dyn_lds, std::atomic<uint64_t>& devices) {
   if (dyn_lds <= 64 * 1024) return QM_OK;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn_lds);
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return qm_fail(QM_ERR_LAUNCH, "no current HIP device");
+  if (devices.load(std::memory_order_acquire) >> dev & 1) return QM_OK;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn_lds);
   if (e != hipSuccess) return qm_fail(QM_ERR_LAUNCH, hipGetErrorString(e));
+  devices.fetch_or(1ull << dev, std::memory_order_release);
   return QM_OK;
 }
 
