@@ -38,14 +38,15 @@ _tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_tor
 def refuse_recording() -> None:
     """Raise where torch records the operations of a call: it would see the output
     made and not what the kernels write into it."""
-    if _tracing_state() is not None or _dispatch_modes() and \
+    if _tracing_state() is not None or \
             torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise RuntimeError("the 4-bit weights' and the experts' operators cannot be traced (torch.jit.trace, make_fx)")
 
 
 def launch(name: str, device, *args) -> None:
     """The entry point ``name`` on ``args`` and the current stream of ``device``."""
-    refuse_recording()
+    if _dispatch_modes() or _tracing_state() is not None:
+        refuse_recording()
     fn, index = getattr(native.load(), name), device.index
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
@@ -120,10 +121,9 @@ class Mx4Weight(SetOnce):
         self._set(data, shape)
 
     def _set(self, data: torch.Tensor, shape: torch.Size) -> None:
-        self.data, self.shape = data, shape
-        self.mats = 1 if len(shape) == 2 else shape[:-2].numel()
-        # the codes are 16 of 17 bytes, the scales behind them
-        self.code_bytes = data.numel() // 17 * 16
+        # (the codes are 16 of 17 bytes, the scales behind them)
+        self.__dict__.update(data=data, shape=shape, mats=1 if len(shape) == 2 else shape[:-2].numel(),
+                             code_bytes=data.numel() // 17 * 16)
 
     # (read from the tensor each time: a copied or loaded weight has memory of its own)
     @property
