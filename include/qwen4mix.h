@@ -502,7 +502,7 @@ int qm_mx4_dequantize(int act_dtype, int mats, int n, int k, const void* codes, 
 int qm_mx4_layout(int to_tiles, int mats, int n, int k, void* codes, void* scales, void* plain_codes,
                   void* plain_scales, hipStream_t stream);
 
-/* The projections of qm_gemv / qm_gemm_rows with 4-bit weights, for any number of
+/* The projections of qm_gemv / qm_gemm_rows with 4-bit weights, for 1 to 1048560
  * activation rows: y[m][j] = sum_k w[j][k] x[m][k], w the values the codes stand
  * for, float sums rounded once to act_dtype.
  *   x [m, k] act_dtype, rows ldx elements apart (ldx >= k, whole 16-byte units;
@@ -516,10 +516,14 @@ int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* codes, const v
 /* ------------------------------------------------------------------------ */
 
 /* The routing of the mixture-of-experts layer (reference/model.py:387-417):
- * logits = x router^T summed in double; ids [rows, top_k] the experts of the
- * largest logits in falling order (equal logits: the lower index first; NaN
- * above every number); weights [rows, top_k] their softmax over all experts, or
- * over the chosen ones when `normalize`.
+ * logits = x router^T; ids [rows, top_k] the experts of the largest logits in
+ * falling order (equal logits: the lower index first; NaN above every number), as
+ * sums in double order them, whatever the number of rows; weights [rows, top_k]
+ * their softmax over all experts, or over the chosen ones when `normalize`. Few rows
+ * take it of the sums in double, many of sums that are float over 128 products at a
+ * time: each logit within (129 2^-23) |x| |router row| (2-norms), but for those that
+ * close to another leading one, which are summed again in double. Exponentials are
+ * floats of a difference in double. Up to 262140 rows.
  *   x [rows, hidden] act_dtype, rows ldx elements apart; router [experts,
  *   hidden]; both 16-byte aligned, hidden a multiple of 32, ldx whole 16-byte
  *   units; experts <= 1024, top_k <= 32. The workspace holds nothing between
@@ -536,7 +540,7 @@ int qm_moe_route(int act_dtype, int rows, int hidden, int experts, int top_k, in
 int qm_tile_weight(int act_dtype, int mats, int n, int k, const void* w, void* tiles, hipStream_t stream);
 
 typedef struct qm_moe_geom {
-  int rows;          /* tokens                                               */
+  int rows;          /* tokens, <= 262140                                    */
   int hidden;        /* width of x and out (a multiple of 32)                 */
   int inter;         /* hidden units of an expert (a multiple of 32)          */
   int experts;       /* routed experts, <= 1024                               */
@@ -568,14 +572,17 @@ typedef struct qm_moe_weights {
   const void* shared_down_scales;
 } qm_moe_weights;
 
-/* Bytes of workspace qm_moe needs; 0 if the geometry is unsupported. */
+/* Bytes of workspace qm_moe needs; 0 if the geometry is unsupported. Beyond 16 rows
+ * most of it is (top_k + shared) rows x hidden floats: 2000 tokens of 9 experts over
+ * 2048 take 0.2 GB, 262140 of them 22 GB; a caller short of memory splits its rows. */
 size_t qm_moe_workspace(const qm_moe_geom* g);
 
 /* A whole mixture-of-experts layer (reference/model.py:387-417):
  *   out[t] = sum_j w[t][j] down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][j]
  *          + sigmoid(x[t] . shared_router) sum_s (the same of shared expert s)
- * with ids and w as qm_moe_route. Products accumulate in float; a pair's weighted
- * hidden row is rounded to act_dtype between them, the output once.
+ * with ids and w as qm_moe_route (the sigmoid of a logit of the same sums). Products
+ * accumulate in float; a pair's weighted hidden row is rounded to act_dtype between
+ * them, the output once.
  *   x [rows, hidden] act, rows ldx elements apart; out [rows, hidden] act; every
  *   pointer 16-byte aligned, scales 4-byte. out may not overlap x. The workspace holds
  *   nothing between calls; calls that overlap need one each. */

@@ -6,9 +6,11 @@
 //
 // A pair is a (token, expert) choice; pair (top_k + shared) t + j is choice j of
 // token t, the shared experts its last ones. The pair's weight multiplies the
-// hidden row in float before that is rounded to the activations' type (the
-// operand of the second product), so the second products add up unweighted, in
-// the order of j.
+// hidden row in float before that is rounded to the activations' type, so the second
+// products add up unweighted, in the order of j. That rounding is the second
+// product's bf16 operand: one MFMA a piece and half of a float row's bytes; it adds as
+// much error as the output's own rounding (relative error of the layer 2.3e-3 where
+// float hidden rows would leave 1.7e-3). Float activations keep float hidden rows.
 #include "moe_internal.h"
 #include "moe_topk.h"
 #include "wgemm.h"
@@ -64,7 +66,7 @@ __device__ __forceinline__ WMat expert_mat(const WMat& m, int e, long tiles, int
 //
 // What bounds it is the weights' way from memory. 8 of 128 experts of 2048 x 512 and
 // a shared one: one token, bf16, 57 MB: logits 3.1 us, up 10 to 11.6 (2 of them the
-// ranking), down 6; 9 tokens, 4-bit, 107 MB: 4.1, table 4.6, up 15 (4.7 TB/s), down
+// ranking), down 6; 9 tokens, 4-bit, 96 MB: 4.2, table 4.6, up 15 (4.2 TB/s), down
 // 11.5. Against the many-token kernels: 8 tokens, 4-bit, 34 for 39 us, 16 tokens 46 and
 // 46, bf16 98 for 108.
 // ---------------------------------------------------------------------------
@@ -87,7 +89,9 @@ struct FewArgs {
   unsigned* down_done; // [output tile] how many have theirs there, cleared before
 };
 
-// choice `lane` of a token and its weight, by one wave
+// choice `lane` of a token and its weight, by one wave. The exponential is a float of a
+// difference taken in double, and so is the sum of up to 32 (or all) of them: a weight
+// is off by some 1e-7 of it, far below the rounding that the hidden row sees.
 template <int PER>
 __device__ __forceinline__ int wave_choose(const double* l, int experts, int top_k, int normalize, int lane, float& weight) {
   long long key;

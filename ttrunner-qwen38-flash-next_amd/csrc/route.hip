@@ -5,7 +5,7 @@
 //
 // The choice is that of the logits summed in double: which experts a token takes
 // then depends on its values alone, not on the number of rows beside it or the
-// order of a float sum, so a verify step routes as the single steps do.
+// order of a float sum: equal rows are routed alike in a verify step and a single one.
 //
 // Few rows form those sums outright, a wave per router row. Many rows take the
 // matrix cores: products of 128 k are summed in float, the sums of 128 in double,
@@ -13,7 +13,10 @@
 //     B = (129 2^-23) |x| |R[e]| + hidden 2^-126      (|.| the 2-norms; the last
 // for products below float's range), and only where two of a token's leading
 // logits come closer than 2 B can the order be another. Those logits alone are
-// summed again in double (about one token in ten of normal rows has such a pair).
+// summed again in double (about one token in ten of normal rows has such a pair). The
+// weights come of the logits as they then are. Their exponentials and sums are floats
+// (of differences in double; 8e-8 of a weight, where a double's would leave the 3e-8
+// of its rounding): what a layer multiplies by them has a float's bits at most.
 #include "moe_internal.h"
 #include "moe_topk.h"
 #include "wgemm.h"

@@ -54,9 +54,10 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool
 
     ids are the experts of the largest logits x router^T in falling order (equal
     ones: the lower index first; NaN above every number), weights their softmax
-    over all experts, or over the chosen ones when ``normalize``. The logits are
-    summed in float64, so that a token's experts do not depend on the rows beside
-    it."""
+    over all experts, or over the chosen ones when ``normalize``. The order is that of
+    sums in float64, so a token's experts do not depend on the rows beside it. Its
+    weights do by their last bits: with many rows they come of logits summed in
+    float, 128 products at a time (include/qwen4mix.h gives the bound)."""
     act = check_input(x, "x")
     _check_router_shape(router)
     _check_router(x, router, top_k)
@@ -207,8 +208,10 @@ class MoeWeights(SetOnce):
 
 
 def moe(x: torch.Tensor, weights: MoeWeights) -> torch.Tensor:
-    """The layer's output for x [..., hidden] (the weights' type), in x's shape:
-    the weighted sum of each token's experts plus its shared experts."""
+    """The layer's output for x [..., hidden] (the weights' type, up to 262140 rows), in
+    x's shape: the weighted sum of each token's experts plus its shared experts. A
+    call's sums differ by their order between 1, 2 to 16 and more rows; its memory
+    grows by (top_k + shared) hidden floats a row."""
     check_input(x, "x")
     _check_router(x, weights.router, weights.top_k)
     device = x.device
