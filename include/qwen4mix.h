@@ -521,8 +521,8 @@ int qm_mx4_linear(int act_dtype, int m, int n, int k, const void* codes, const v
  * sums in double order them, whatever the number of rows; weights [rows, top_k]
  * their softmax over all experts, or over the chosen ones when `normalize`. Few rows
  * take it of the sums in double, many of sums that are float over 128 products at a
- * time: each logit within (129 2^-23) |x| |router row| (2-norms), but for those that
- * close to another leading one, which are summed again in double. Exponentials are
+ * time: each logit within (129 2^-23) |x| |router row| + hidden 2^-126 (2-norms), but
+ * for those that close to another leading one, which are summed again in double. Exponentials are
  * floats of a difference in double. Up to 262140 rows.
  *   x [rows, hidden] act_dtype, rows ldx elements apart; router [experts,
  *   hidden]; both 16-byte aligned, hidden a multiple of 32, ldx whole 16-byte

@@ -309,7 +309,8 @@ int launch_gemm(const Mx4LinearArgs<T>& A, hipStream_t stream) {
 //     10.4 / 13.4 / 15.4 / 23.0 / 35, 400 rows (208) 16.6 / 13.6 / 15.3 / 19.7 / 35
 //     Wide weights, whose few rows make as many workgroups: up to 8 rows stay with the
 //     few-row kernel, up to 32 with tiles of 32 (few-row / 256 x 32 / 256 x 64, x 2048:
-//     65536, 1 row 16.8 / 19.3 / 20.7; 151936: 1 row 33.1 / 35.6 / 47.4, 8 rows 34.9 /
+//     65536, 1 row 16.8 / 19.3 / 20.7; 98304, 1 row 23.2 / 23.9 / 33.2, 8 rows 24.8 /
+//     23.9 / 32.9, 16 rows 26.6 / 24.0 / 34.5; 151936: 1 row 33.1 / 35.6 / 47.4, 8 rows 34.9 /
 //     35.9 / 49.7, 16 rows 38.6 / 36.6 / 52.1, 32 rows 60 / 40.8 / 56.8; 262144: 1 row
 //     51.7 / 61.8 / 63.3, 8 rows 54.0 / 63.1 / 66.0, 32 rows 120 / 66.2 / 73.0)
 //   float   256 x 32 tiles from 512 workgroups on (2000 rows of 9856 x 2048: 283
